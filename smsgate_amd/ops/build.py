@@ -59,6 +59,13 @@ def build(force: bool = False, verbose: bool = False, extra: Optional[List[str]]
         # attention kernels one wave of occupancy (scripts/kernel_resources.py)
         "-mllvm",
         "-amdgpu-mfma-vgpr-form=1",
+        # no packed-fp32 instructions (v_pk_fma_f32 and its like, which -O3 forms from
+        # ordinary float code): some of their forms have given wrong results now and then.
+        # The host pass does not know the feature and says so; that warning is harmless
+        "-Xclang",
+        "-target-feature",
+        "-Xclang",
+        "-packed-fp32-ops",
         *(extra or []),
         *[str(s) for s in sources()],
         "-o",

@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(256) rmsnorm_residual_kernel(const uint16_t* _
   for (int k = 0; k < RMS_MAXV; ++k) {
     const int c = lane + k * WAVE;
     if (c < nvec) {
+#pragma clang fp contract(off)  // squares are rounded before they are summed
       unpack8(rv[k], a[k]);
       if (x4) {
         float b[8];

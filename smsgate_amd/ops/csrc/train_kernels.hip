@@ -170,6 +170,9 @@ __global__ void __launch_bounds__(256) rope_split_kernel(uint16_t* __restrict__ 
   }
   const int jj = j & (HD - 1);
   if (DIR > 0) {
+    // (here and below) both products of a rotation are rounded on their own, whatever the
+    // compiler's vectoriser makes of them
+#pragma clang fp contract(off)
     float o;
     if (rot) {
       const float c = cos_t[t * HD + jj], s = sin_t[t * HD + jj];
@@ -181,6 +184,7 @@ __global__ void __launch_bounds__(256) rope_split_kernel(uint16_t* __restrict__ 
     const uint16_t ob = tk_f2bf(o);
     for (int r = 0; r < copies; ++r) dst[r * hstride + j] = ob;
   } else {  // adjoint: sum of the copies' gradients, then rotation by -theta
+#pragma clang fp contract(off)
     if (rot) {
       const float c = cos_t[t * HD + jj], s = sin_t[t * HD + jj];
       float d1 = 0.f, d2 = 0.f;
