@@ -34,11 +34,13 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 from .extractor import ExtractorWeights, _rope_tables
 
-__all__ = ["fused_forward", "rms_norm", "rope_split", "swiglu", "attention", "available", "ATTN_MAX_T"]
+__all__ = ["fused_forward", "rms_norm", "rope_split", "swiglu", "attention", "available", "ATTN_MAX_T",
+           "embed_lookup"]
 
 
 def available(device) -> bool:
@@ -184,6 +186,86 @@ class _Attention(torch.autograd.Function):
                                      dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dsum.data_ptr(), B,
                                      T, nh, nkv, float(ctx.scale), _st()), "attn_train_bwd")
         return dq, dk, dv, None
+
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # csrc/embed_kernels.hip
+
+
+def _run(dev: torch.device, name: str, fn, *args) -> None:
+    """Launches ``fn`` on ``dev`` (current or not), on that device's current stream."""
+    if dev.index == torch.cuda.current_device():
+        _ok(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+    else:
+        with torch.cuda.device(dev):
+            _ok(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def _on_gpu(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    first = tensors[0]
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device != first.device):
+            raise ValueError(f"{name}: every tensor must be on the same GPU")
+
+
+def _vec16(H: int, *tensors: torch.Tensor) -> int:
+    """1 when rows of ``H`` elements of every tensor can be read 16 bytes at a time."""
+    return int(H * tensors[0].element_size() % 16 == 0 and all(t.data_ptr() % 16 == 0 for t in tensors))
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table: torch.Tensor, ids: torch.Tensor, add: Optional[torch.Tensor], scale: float):
+        V, H = table.shape
+        n = ids.numel()
+        table = table.contiguous()
+        ids = ids.contiguous()
+        add = None if add is None else add.contiguous()
+        x = torch.empty(*ids.shape, H, dtype=table.dtype, device=table.device)
+        ctx.save_for_backward(ids, add)
+        ctx.dims = (n, V, H, float(scale))
+        if n:
+            _run(table.device, "embed_fwd", _lib().sg_embed_fwd, ids.data_ptr(), ops._p(add),
+                 int(ids.dtype == torch.int64), table.data_ptr(), x.data_ptr(), n, V, H, float(scale),
+                 _DTYPES[table.dtype], _vec16(H, table, x))
+        return x
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dx: torch.Tensor):
+        ids, add = ctx.saved_tensors
+        n, V, H, scale = ctx.dims
+        if not n:
+            return torch.zeros(V, H, dtype=dx.dtype, device=dx.device), None, None, None
+        dx = dx.contiguous()
+        dt = torch.empty(V, H, dtype=dx.dtype, device=dx.device)
+        lib = _lib()
+        units = lib.sg_embed_grad_ws(n if add is None else 2 * n, V, H)  # of 256 bytes
+        ws = torch.empty(units * 64, dtype=torch.int32, device=dx.device) if units else None
+        _run(dx.device, "embed_grad", lib.sg_embed_grad, ids.data_ptr(), ops._p(add), int(ids.dtype == torch.int64),
+             dx.data_ptr(), dt.data_ptr(), n, V, H, scale, _DTYPES[dx.dtype], _vec16(H, dx, dt), ops._p(ws), units)
+        return dt, None, None, None
+
+
+def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch.Tensor] = None, *,
+                 scale: float = 1.0) -> torch.Tensor:
+    """``scale * (table[ids] + table[add_ids])`` as ``[*ids.shape, H]`` in the table's type
+    (csrc/embed_kernels.hip), differentiable in ``table``.
+
+    ``ids``: int32 or int64, any shape.  ``table`` [V, H]: fp32, bf16 or fp16.  ``add_ids``
+    (``ids``' shape and type): a second row added to each position, negative = none (the
+    span formats' pointer rows).  The sum is taken and scaled in fp32 and rounded once.  The
+    table's gradient sums the positions of each id in fp32, in their order: the same bits
+    every run.  An id outside [0, V) (``add_ids``: above it) gives a NaN row and no gradient."""
+    if table.dim() != 2 or table.dtype not in _DTYPES:
+        raise TypeError("embed_lookup: table must be fp32, bf16 or fp16 [V, H]")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("embed_lookup: ids must be int32 or int64")
+    if add_ids is not None and (add_ids.shape != ids.shape or add_ids.dtype != ids.dtype):
+        raise ValueError("embed_lookup: add_ids must have the shape and type of ids")
+    if min(table.shape) < 1 or table.shape[0] >= 1 << 30 or ids.numel() >= 1 << 30:
+        raise ValueError("embed_lookup: 1 <= V < 2^30, H >= 1, fewer than 2^30 ids")
+    _on_gpu("embed_lookup", table, ids, add_ids)
+    return _Embed.apply(table, ids, add_ids, scale)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -> torch.Tensor:

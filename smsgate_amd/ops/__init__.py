@@ -159,6 +159,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.sg_swiglu_bwd.argtypes = [_vp, _vp, _vp, _c_int, _c_int, _vp]
     lib.sg_attn_train_fwd.argtypes = [_vp] * 5 + [_c_int] * 4 + [_c_float, _vp]
     lib.sg_attn_train_bwd.argtypes = [_vp] * 10 + [_c_int] * 4 + [_c_float, _vp]
+    # token embedding and its gradient (csrc/embed_kernels.hip)
+    lib.sg_embed_fwd.argtypes = [_vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _vp]
+    lib.sg_embed_fwd.restype = _c_int
+    lib.sg_embed_grad_ws.argtypes = [_c_int, _c_int, _c_int]
+    lib.sg_embed_grad_ws.restype = _c_int
+    lib.sg_embed_grad.argtypes = [_vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _vp,
+                                  _c_int, _vp]
+    lib.sg_embed_grad.restype = _c_int
     for fn in (lib.sg_rms_fwd, lib.sg_rms_bwd, lib.sg_rope_split, lib.sg_swiglu_fwd, lib.sg_swiglu_bwd,
                lib.sg_attn_train_fwd, lib.sg_attn_train_bwd):
         fn.restype = _c_int
