@@ -191,13 +191,16 @@ class _Attention(torch.autograd.Function):
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # csrc/embed_kernels.hip
 
 
-def _run(dev: torch.device, name: str, fn, *args) -> None:
-    """Launches ``fn`` on ``dev`` (current or not), on that device's current stream."""
-    if dev.index == torch.cuda.current_device():
-        _ok(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+def _run(dev: int, name: str, fn, *args) -> None:
+    """Launches ``fn`` on device ``dev`` (current or not), on that device's current stream
+    (its raw handle: a Stream object costs as much host time as the launch)."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            _ok(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        raise RuntimeError(f"{name} failed (rc={rc})")
 
 
 def _on_gpu(name: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -209,40 +212,43 @@ def _on_gpu(name: str, *tensors: Optional[torch.Tensor]) -> None:
 
 def _vec16(H: int, *tensors: torch.Tensor) -> int:
     """1 when rows of ``H`` elements of every tensor can be read 16 bytes at a time."""
-    return int(H * tensors[0].element_size() % 16 == 0 and all(t.data_ptr() % 16 == 0 for t in tensors))
+    ptrs = 0
+    for t in tensors:
+        ptrs |= t.data_ptr()
+    return int((ptrs | H * tensors[0].element_size()) % 16 == 0)
 
 
 class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table: torch.Tensor, ids: torch.Tensor, add: Optional[torch.Tensor], scale: float):
         V, H = table.shape
-        n = ids.numel()
-        table = table.contiguous()
-        ids = ids.contiguous()
+        n, dev, code, is64 = ids.numel(), table.get_device(), _DTYPES[table.dtype], int(ids.dtype == torch.int64)
+        table, ids = table.contiguous(), ids.contiguous()
         add = None if add is None else add.contiguous()
         x = torch.empty(*ids.shape, H, dtype=table.dtype, device=table.device)
-        ctx.save_for_backward(ids, add)
-        ctx.dims = (n, V, H, float(scale))
+        lib = _lib()
         if n:
-            _run(table.device, "embed_fwd", _lib().sg_embed_fwd, ids.data_ptr(), ops._p(add),
-                 int(ids.dtype == torch.int64), table.data_ptr(), x.data_ptr(), n, V, H, float(scale),
-                 _DTYPES[table.dtype], _vec16(H, table, x))
+            _run(dev, "embed_fwd", lib.sg_embed_fwd, ids.data_ptr(), ops._p(add), is64, table.data_ptr(),
+                 x.data_ptr(), n, V, H, scale, code, _vec16(H, table, x))
+        ctx.save_for_backward(ids, add)
+        # all that the gradient's launch needs but the pointers: autograd's thread pays
+        # more for each Python step than the caller's
+        ctx.plan = (lib.sg_embed_grad, dev, n, V, H, scale, code, is64,
+                    lib.sg_embed_grad_ws(n if add is None else 2 * n, V, H))
         return x
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dx: torch.Tensor):
-        ids, add = ctx.saved_tensors
-        n, V, H, scale = ctx.dims
+        fn, dev, n, V, H, scale, code, is64, units = ctx.plan
         if not n:
-            return torch.zeros(V, H, dtype=dx.dtype, device=dx.device), None, None, None
+            return dx.new_zeros(V, H), None, None, None
+        ids, add = ctx.saved_tensors
         dx = dx.contiguous()
-        dt = torch.empty(V, H, dtype=dx.dtype, device=dx.device)
-        lib = _lib()
-        units = lib.sg_embed_grad_ws(n if add is None else 2 * n, V, H)  # of 256 bytes
-        ws = torch.empty(units * 64, dtype=torch.int32, device=dx.device) if units else None
-        _run(dx.device, "embed_grad", lib.sg_embed_grad, ids.data_ptr(), ops._p(add), int(ids.dtype == torch.int64),
-             dx.data_ptr(), dt.data_ptr(), n, V, H, scale, _DTYPES[dx.dtype], _vec16(H, dx, dt), ops._p(ws), units)
+        dt = dx.new_empty(V, H)
+        ws = dx.new_empty(units * 64, dtype=torch.int32) if units else None  # units of 256 bytes
+        _run(dev, "embed_grad", fn, ids.data_ptr(), ops._p(add), is64, dx.data_ptr(), dt.data_ptr(), n, V, H, scale,
+             code, _vec16(H, dx, dt), ops._p(ws), units)
         return dt, None, None, None
 
 
@@ -265,7 +271,7 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch
     if min(table.shape) < 1 or table.shape[0] >= 1 << 30 or ids.numel() >= 1 << 30:
         raise ValueError("embed_lookup: 1 <= V < 2^30, H >= 1, fewer than 2^30 ids")
     _on_gpu("embed_lookup", table, ids, add_ids)
-    return _Embed.apply(table, ids, add_ids, scale)
+    return _Embed.apply(table, ids, add_ids, float(scale))
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -> torch.Tensor:
