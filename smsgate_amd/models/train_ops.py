@@ -28,6 +28,7 @@ losses and gradients).  CPU / no-library: reference_forward.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import math
 import os
 from typing import Optional
@@ -40,7 +41,7 @@ from .. import ops
 from .extractor import ExtractorWeights, _rope_tables
 
 __all__ = ["fused_forward", "rms_norm", "rope_split", "swiglu", "attention", "available", "ATTN_MAX_T",
-           "embed_lookup"]
+           "embed_lookup", "tiled_attention"]
 
 
 def available(device) -> bool:
@@ -276,6 +277,79 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -> torch.Tensor:
     return _Attention.apply(q, k, v, scale)
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [B, heads, T, D] itself when its rows can be read 16 bytes at a time, else a copy."""
+    if t.stride(3) == 1 and (t.stride(0) | t.stride(1) | t.stride(2)) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.contiguous()
+
+
+class _TiledAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, scale: float, causal: bool):
+        B, nh, T, D = q.shape
+        nkv, dev, fp16 = k.shape[1], q.get_device(), int(q.dtype == torch.float16)
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        lengths = None if lengths is None else lengths.contiguous()
+        lib = _lib()
+        rows = lib.sg_attn_rows(T)
+        out = torch.empty(B, T, nh * D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(B, nh, rows, dtype=torch.float32, device=q.device)
+        strides = (ctypes.c_long * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        dims = (B, T, nh, nkv, D, int(causal), fp16, scale)
+        _run(dev, "attn_fwd", lib.sg_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), ops._p(lengths),
+             out.data_ptr(), lse.data_ptr(), strides, *dims)
+        ctx.save_for_backward(q, k, v, lengths, out, lse)
+        words = B * nh * rows + 256 * fp16 + (2 * B * nh * T * D if lib.sg_attn_split(B, T, nh, nkv) else 0)
+        ctx.plan = (lib.sg_attn_bwd, dev, strides, dims, words)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout: torch.Tensor):
+        q, k, v, lengths, out, lse = ctx.saved_tensors
+        fn, dev, strides, dims, words = ctx.plan
+        dout = dout.contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        ws = lse.new_empty(words)
+        _run(dev, "attn_bwd", fn, q.data_ptr(), k.data_ptr(), v.data_ptr(), ops._p(lengths), out.data_ptr(),
+             lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), strides, *dims)
+        return dq, dk, dv, None, None, None
+
+
+def tiled_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None, *,
+                    causal: bool = True, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Grouped-query attention of a batch in matrix instructions
+    (csrc/attn_grad_kernels.hip), any length, differentiable in q, k and v.
+
+    ``q`` [B, nh, T, D], ``k`` / ``v`` [B, nkv, T, D]: bf16 or fp16, D 64 or 128, nh a
+    multiple of nkv (query head h reads key head ``h // (nh // nkv)``), any strides.
+    ``scale``: > 0, default ``D ** -0.5``.  ``causal``: query i sees keys up to i.
+    ``lengths`` (int32 [B]): sequence b is its first ``lengths[b]`` rows (clamped to 0..T);
+    the rows behind are zero in the result and in every gradient, and what they hold in q,
+    k, v and the incoming gradient has no effect, infinities and NaN included.  Returns
+    [B, T, nh * D] (the o-projection's input).  Probabilities are recomputed in the
+    backward pass and nothing of size T x T is stored; every sum has a fixed order."""
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("tiled_attention: q, k and v must all be bf16 or all fp16")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or min(q.shape) < 1 or min(k.shape) < 1:
+        raise ValueError("tiled_attention: q [B, nh, T, D], k and v [B, nkv, T, D], none of them empty")
+    B, nh, T, D = q.shape
+    if k.shape[0] != B or k.shape[2:] != (T, D) or nh % k.shape[1] or D not in (64, 128):
+        raise ValueError("tiled_attention: k and v need q's batch, length and width (64 or 128), and nh % nkv == 0")
+    if T > 1 << 24 or B * nh > 1 << 20 or B * nh * ((T + 31) // 32) > 0x7FFFFFFF:
+        raise ValueError("tiled_attention: T <= 2^24, B * nh <= 2^20, fewer than 2^31 tiles")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("tiled_attention: scale must be finite and above 0")
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,)):
+        raise ValueError("tiled_attention: lengths must be int32 [B]")
+    _on_gpu("tiled_attention", q, k, v, lengths)
+    return _TiledAttention.apply(q, k, v, lengths, scale, bool(causal))
 
 
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:

@@ -23,3 +23,36 @@ def _ids(*shape, dtype=torch.long):
 def test_embed_lookup_refuses(ids, table, add, err):
     with pytest.raises(err, match="embed_lookup"):
         train_ops.embed_lookup(ids, table, add)
+
+
+def _qkv(B=2, T=5, nh=4, nkv=2, D=64, dtype=torch.bfloat16):
+    return torch.zeros(B, nh, T, D, dtype=dtype), torch.zeros(B, nkv, T, D, dtype=dtype), \
+        torch.zeros(B, nkv, T, D, dtype=dtype)
+
+
+@pytest.mark.parametrize("change,kw,err", [
+    (dict(dtype=torch.float32), {}, TypeError),
+    (dict(D=80), {}, ValueError),
+    (dict(nh=3), {}, ValueError),                                            # heads that do not divide
+    (dict(T=0), {}, ValueError),
+    (dict(B=0), {}, ValueError),
+    ({}, dict(scale=0.0), ValueError),
+    ({}, dict(scale=-1.0), ValueError),
+    ({}, dict(scale=float("nan")), ValueError),
+    ({}, dict(scale=float("inf")), ValueError),
+    ({}, dict(lengths=torch.zeros(2, dtype=torch.int64)), ValueError),
+    ({}, dict(lengths=torch.zeros(3, dtype=torch.int32)), ValueError),
+    ({}, {}, ValueError),                                                    # not on a GPU
+])
+def test_tiled_attention_refuses(change, kw, err):
+    with pytest.raises(err, match="tiled_attention"):
+        train_ops.tiled_attention(*_qkv(**change), **kw)
+
+
+def test_tiled_attention_refuses_mismatched_operands():
+    q, k, v = _qkv()
+    for bad in ((q, k[:1], v[:1]), (q, k[:, :, :4], v[:, :, :4]), (q, k, v[:, :1]), (q[0], k, v), (q, k[0], v[0])):
+        with pytest.raises(ValueError, match="tiled_attention"):
+            train_ops.tiled_attention(*bad)
+    with pytest.raises(TypeError, match="tiled_attention"):
+        train_ops.tiled_attention(q, k.half(), v)
