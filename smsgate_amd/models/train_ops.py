@@ -296,12 +296,14 @@ class _TiledAttention(torch.autograd.Function):
         lib = _lib()
         rows = lib.sg_attn_rows(T)
         out = torch.empty(B, T, nh * D, dtype=q.dtype, device=q.device)
+        # what rounding took from out, for the backward's D (none: no gradient will be asked)
+        olo = torch.empty_like(out) if any(ctx.needs_input_grad[:3]) else None
         lse = torch.empty(B, nh, rows, dtype=torch.float32, device=q.device)
         strides = (ctypes.c_long * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
         dims = (B, T, nh, nkv, D, int(causal), fp16, scale)
         _run(dev, "attn_fwd", lib.sg_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), ops._p(lengths),
-             out.data_ptr(), lse.data_ptr(), strides, *dims)
-        ctx.save_for_backward(q, k, v, lengths, out, lse)
+             out.data_ptr(), ops._p(olo), lse.data_ptr(), strides, *dims)
+        ctx.save_for_backward(q, k, v, lengths, out, olo, lse)
         words = B * nh * rows + 256 * fp16 + (2 * B * nh * T * D if lib.sg_attn_split(B, T, nh, nkv) else 0)
         ctx.plan = (lib.sg_attn_bwd, dev, strides, dims, words)
         return out
@@ -309,7 +311,7 @@ class _TiledAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: torch.Tensor):
-        q, k, v, lengths, out, lse = ctx.saved_tensors
+        q, k, v, lengths, out, olo, lse = ctx.saved_tensors
         fn, dev, strides, dims, words = ctx.plan
         dout = dout.contiguous()
         if dout.data_ptr() % 16:
@@ -317,7 +319,7 @@ class _TiledAttention(torch.autograd.Function):
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         ws = lse.new_empty(words)
         _run(dev, "attn_bwd", fn, q.data_ptr(), k.data_ptr(), v.data_ptr(), ops._p(lengths), out.data_ptr(),
-             lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), strides, *dims)
+             olo.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), strides, *dims)
         return dq, dk, dv, None, None, None
 
 

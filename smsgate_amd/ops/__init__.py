@@ -170,8 +170,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     # attention of whole sequences and its gradients (csrc/attn_grad_kernels.hip)
     lib.sg_attn_rows.argtypes = [_c_int]
     lib.sg_attn_split.argtypes = [_c_int] * 4
-    lib.sg_attn_fwd.argtypes = [_vp] * 7 + [_c_int] * 7 + [_c_float, _vp]
-    lib.sg_attn_bwd.argtypes = [_vp] * 12 + [_c_int] * 7 + [_c_float, _vp]
+    lib.sg_attn_fwd.argtypes = [_vp] * 8 + [_c_int] * 7 + [_c_float, _vp]
+    lib.sg_attn_bwd.argtypes = [_vp] * 13 + [_c_int] * 7 + [_c_float, _vp]
     for fn in (lib.sg_attn_rows, lib.sg_attn_split, lib.sg_attn_fwd, lib.sg_attn_bwd):
         fn.restype = _c_int
     for fn in (lib.sg_rms_fwd, lib.sg_rms_bwd, lib.sg_rope_split, lib.sg_swiglu_fwd, lib.sg_swiglu_bwd,
