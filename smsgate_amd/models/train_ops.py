@@ -41,7 +41,7 @@ from .. import ops
 from .extractor import ExtractorWeights, _rope_tables
 
 __all__ = ["fused_forward", "rms_norm", "rope_split", "swiglu", "attention", "available", "ATTN_MAX_T",
-           "embed_lookup", "tiled_attention"]
+           "embed_lookup", "tiled_attention", "lm_loss"]
 
 
 def available(device) -> bool:
@@ -352,6 +352,81 @@ def tiled_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
         raise ValueError("tiled_attention: lengths must be int32 [B]")
     _on_gpu("tiled_attention", q, k, v, lengths)
     return _TiledAttention.apply(q, k, v, lengths, scale, bool(causal))
+
+
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and on a 16-byte border (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _LmLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, table, labels, mode: int, ignore: int):
+        V, H = table.shape
+        N, dev, fp16, is64 = labels.numel(), h.get_device(), int(h.dtype == torch.float16), int(
+            labels.dtype == torch.int64)
+        h, table, labels = _aligned(h), _aligned(table), labels.contiguous()
+        lib = _lib()
+        plan = (ctypes.c_int * 5)()
+        _ok(lib.sg_loss_plan(N, V, H, plan), "loss_plan")
+        hc = h.new_empty(plan[0], plan[1])
+        state = torch.empty(plan[2] * 64, dtype=torch.int32, device=h.device)
+        ws = torch.empty(plan[3] * 64, dtype=torch.float32, device=h.device)
+        loss = torch.empty(labels.shape if mode == 2 else (), dtype=torch.float32, device=h.device)
+        _run(dev, "loss_fwd", lib.sg_loss_fwd, h.data_ptr(), table.data_ptr(), labels.data_ptr(), is64, ignore,
+             hc.data_ptr(), state.data_ptr(), ws.data_ptr(), loss.data_ptr(), N, V, H, mode, fp16)
+        ctx.save_for_backward(hc, table, state)
+        ctx.plan = (lib.sg_loss_bwd, dev, h.shape, (N, V, H, mode, fp16), plan[4] * 64)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        hc, table, state = ctx.saved_tensors
+        fn, dev, shape, dims, words = ctx.plan
+        g = g.contiguous()
+        dh = hc.new_empty(shape) if ctx.needs_input_grad[0] else None
+        dt = torch.empty_like(table) if ctx.needs_input_grad[1] else None
+        ws = g.new_empty(words)
+        _run(dev, "loss_bwd", fn, hc.data_ptr(), table.data_ptr(), state.data_ptr(), g.data_ptr(), ws.data_ptr(),
+             ops._p(dh), ops._p(dt), *dims)
+        return dh, dt, None, None, None
+
+
+def lm_loss(h: torch.Tensor, table: torch.Tensor, labels: torch.Tensor, *, reduction: str = "mean",
+            ignore_index: int = -100) -> torch.Tensor:
+    """Softmax cross entropy of ``h @ table.T`` against ``labels`` (csrc/loss_kernels.hip),
+    differentiable in ``h`` and ``table``, without a matrix of logits: the forward keeps
+    tiles of them in registers, the backward recomputes them a piece of the vocabulary at a
+    time.
+
+    ``h`` [..., H] and ``table`` [V, H]: both bf16 or both fp16, H a multiple of 8 (masters
+    in fp32 are cast by the caller, as autocast does).  ``labels`` [...]: int32 or int64.
+    Rows of label ``ignore_index`` cost no product: they are left out by a list built on the
+    GPU.  ``reduction``: ``mean`` over the labelled rows (none labelled: NaN, gradients 0),
+    ``sum``, or ``none`` (fp32 per row, 0 where ignored).  A label outside [0, V) makes its
+    row's loss NaN, and the gradients that take part in it.  Sums are fp32 in a fixed order."""
+    if h.dtype not in (torch.bfloat16, torch.float16) or table.dtype != h.dtype:
+        raise TypeError("lm_loss: h and table must both be bf16 or both fp16")
+    if labels.dtype not in (torch.int32, torch.int64):
+        raise TypeError("lm_loss: labels must be int32 or int64")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"lm_loss: reduction {reduction!r}: mean | sum | none")
+    if h.dim() < 1 or table.dim() != 2 or h.shape[-1] != table.shape[1] or labels.shape != h.shape[:-1]:
+        raise ValueError("lm_loss: h [..., H], table [V, H] and labels [...] do not fit")
+    V, H = table.shape
+    N = labels.numel()
+    if not (1 <= N <= 1 << 24 and 1 <= V <= 1 << 24 and 8 <= H <= 1 << 14) or H % 8 \
+            or ((N + 255) // 64) * ((V + 255) // 64) > 0x7FFFFFFF:
+        raise ValueError("lm_loss: 1 to 2^24 rows and ids, H a multiple of 8 up to 2^14, fewer than 2^31 tiles")
+    if not -(1 << 31) <= ignore_index < 1 << 31:
+        raise ValueError("lm_loss: ignore_index must fit 32 bits")
+    _on_gpu("lm_loss", h, table, labels)
+    return _LmLoss.apply(h, table, labels, _REDUCTIONS[reduction], int(ignore_index))
 
 
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:

@@ -174,6 +174,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.sg_attn_bwd.argtypes = [_vp] * 13 + [_c_int] * 7 + [_c_float, _vp]
     for fn in (lib.sg_attn_rows, lib.sg_attn_split, lib.sg_attn_fwd, lib.sg_attn_bwd):
         fn.restype = _c_int
+    # vocabulary cross entropy and its gradients (csrc/loss_kernels.hip)
+    lib.sg_loss_plan.argtypes = [_c_int] * 3 + [_vp]
+    lib.sg_loss_fwd.argtypes = [_vp] * 3 + [_c_int] * 2 + [_vp] * 4 + [_c_int] * 5 + [_vp]
+    lib.sg_loss_bwd.argtypes = [_vp] * 7 + [_c_int] * 5 + [_vp]
+    for fn in (lib.sg_loss_plan, lib.sg_loss_fwd, lib.sg_loss_bwd):
+        fn.restype = _c_int
     for fn in (lib.sg_rms_fwd, lib.sg_rms_bwd, lib.sg_rope_split, lib.sg_swiglu_fwd, lib.sg_swiglu_bwd,
                lib.sg_attn_train_fwd, lib.sg_attn_train_bwd):
         fn.restype = _c_int

@@ -1,0 +1,677 @@
+// smsgate_amd — softmax cross entropy of hidden states over the rows of the embedding, and
+// the gradients of both, without a [rows, vocabulary] matrix of logits (gfx950).
+//
+//   z = h E^T,  L_i = logsumexp z_i,  loss_i = L_i - z_i[y_i]
+//   d_i[v] = w_i (exp(z_i[v] - L_i) - [v = y_i]),  dh = f d E,  dE = f d^T h
+//
+// h [N, H] and E [V, H] in bf16 or fp16, H a multiple of 8, any N and V.  Rows whose label
+// is ignore_index are left out before any product: loss_rows lists the others, loss_gather
+// copies them together ([Mp][Hp], zero behind the last row and column), and every later
+// block reads the count from the device and ends at once behind it (an SMS batch labels
+// about a third of its positions).
+//
+//   forward   loss_gemm<0>: a tile's logits stay in the accumulators; each row's maximum
+//             and sum of exponentials over the tile go out (8 bytes a row and tile);
+//             loss_join: L and loss, with z_i[y_i] as a dot product of its own
+//   backward  per piece of the vocabulary: loss_gemm<1> recomputes the tile's logits and
+//             writes d in the inputs' type; loss_gemm<2>: the piece's rows of dE;
+//             loss_gemm<3>: dh's share, fp32, the piece's columns split over blocks;
+//             loss_dh sums the shares in order and puts the rows back (ignored: zeros)
+//
+// Four products of 2 n V H flops where keeping the logits would need three: z is needed in
+// fp32 (its rounding to 16 bits would put errors of per cents into exp), and storing it
+// costs more memory time at H = 576 than multiplying again.  d is rounded to the inputs'
+// type as an operand (as the gradient of such logits is under autocast); fp16 holds
+// nothing under 2^-24, so there d is scaled by 2^10 (|d| <= 1) and f takes it out.  Every
+// other sum, L and dh's shares are fp32; no float atomics, every sum has a fixed order.
+//
+// Products: v_mfma_f32_32x32x16, result in lane l: column l & 31 (the "lane" side: a hidden
+// row, or a vocabulary row for dE), rows (r & 3) + 8 (r >> 2) + 4 (l >> 5) (the "register"
+// side).  Operands whose k runs along memory are read from LDS as rows, others by
+// transposing reads (ds_read_b64_tr_b16) of tiles kept as they lie in memory, so no
+// transposed copy of E, h or d exists.  Tiles come by DMA (global_load_lds) into two
+// buffers, one barrier a 64-wide step; 16-byte chunks are XORed by row against bank
+// conflicts.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lk_lds_t;
+typedef __attribute__((address_space(3))) s16x4* lk_tr_t;
+
+constexpr float LK_LOG2E = 1.4426950408889634f;
+constexpr int LK_K = 64;         // k-values of a staged tile
+constexpr int LK_PAD = 256;      // rows and pieces are padded to whole tiles
+constexpr float LK_FP16 = 1024.f;  // factor on d in fp16
+
+__device__ const uint4 lk_zero = {0, 0, 0, 0};
+
+struct LossArgs {
+  const uint16_t *h, *table;
+  const void* labels;
+  uint16_t *hc, *d, *dh, *dtable;
+  int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; [1]
+  float *lse, *rl, *loss, *w;       // [Mp] L in log2; [Mp] loss; out; [Mp] row weights or null
+  float2* part;                     // [v tiles][Mp] (maximum, sum of exp(z - maximum))
+  float* share;                     // [splits][Mp][Hp]
+  const float *g, *gmax;            // incoming gradient; none: its largest magnitude
+  long ignore;
+  int N, V, H, Mp, Hp, is64, mode;  // mode 0 mean, 1 sum, 2 none
+  int v0, vn, ldd;                  // piece: first row, rows (of them < V - v0 real), stride of d
+  int splits, first;
+};
+
+template <bool BF>
+__device__ __forceinline__ f32x16 lk_mma(u16x8 a, u16x8 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+template <bool BF>
+__device__ __forceinline__ uint16_t lk_round(float x) {
+  if constexpr (BF) {
+    const __bf16 b = (__bf16)x;
+    return __builtin_bit_cast(uint16_t, b);
+  } else {
+    const _Float16 b = (_Float16)x;
+    return __builtin_bit_cast(uint16_t, b);
+  }
+}
+
+template <bool BF>
+__device__ __forceinline__ float lk_float(uint16_t x) {
+  if constexpr (BF)
+    return __uint_as_float((uint32_t)x << 16);
+  else
+    return (float)__builtin_bit_cast(_Float16, x);
+}
+
+template <bool BF>
+__device__ __forceinline__ uint2 lk_pack4(float a, float b, float c, float d) {
+  return make_uint2((uint32_t)lk_round<BF>(a) | ((uint32_t)lk_round<BF>(b) << 16),
+                    (uint32_t)lk_round<BF>(c) | ((uint32_t)lk_round<BF>(d) << 16));
+}
+
+__device__ __forceinline__ float lk_max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float lk_sum_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ float lk_exp(float x) { return __builtin_amdgcn_exp2f(x * LK_LOG2E); }
+
+__device__ __forceinline__ int lk_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+// ---- rows with a label -----------------------------------------------------------------
+// One block: places of the labelled rows, in order.  A label outside [0, V) becomes -2 (its
+// loss and gradients are NaN).
+__global__ void __launch_bounds__(1024) loss_rows_kernel(LossArgs a) {
+  __shared__ int part[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int base = 0;
+  for (int i0 = 0; i0 < a.N; i0 += 8192) {
+    long y[8];
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + 8 * tid + k;
+      y[k] = i < a.N ? (a.is64 ? reinterpret_cast<const long*>(a.labels)[i]
+                               : (long)reinterpret_cast<const int*>(a.labels)[i])
+                     : a.ignore;
+      n += y[k] != a.ignore;
+    }
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += t;
+    }
+    if (lane == 63) part[wave] = inc;
+    __syncthreads();
+    int at = base + inc - n, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) at += part[w];
+      all += part[w];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + 8 * tid + k;
+      if (i >= a.N) continue;
+      const bool on = y[k] != a.ignore;
+      a.pos[i] = on ? at : -1;
+      if (on) {
+        a.rows[at] = i;
+        a.lab[at] = y[k] >= 0 && y[k] < a.V ? (int)y[k] : -2;
+        ++at;
+      } else if (a.mode == 2) {
+        a.loss[i] = 0.f;
+      }
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) a.cnt[0] = base;
+}
+
+// hc[m] = h[rows[m]], zeros behind the last row (up to a whole tile) and column; 16 bytes a thread
+__global__ void __launch_bounds__(256) loss_gather_kernel(LossArgs a) {
+  const int nch = a.Hp / 8, cnt = a.cnt[0];
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(i / nch), c = (int)(i - (long)m * nch);
+  if (m >= (cnt + LK_PAD - 1) / LK_PAD * LK_PAD || m >= a.Mp) return;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (m < cnt && 8 * c < a.H) v = *reinterpret_cast<const uint4*>(a.h + (size_t)a.rows[m] * a.H + 8 * c);
+  *reinterpret_cast<uint4*>(a.hc + (size_t)m * a.Hp + 8 * c) = v;
+}
+
+// ---- products --------------------------------------------------------------------------
+// Row operand: row `row` of a [rows][64] tile, k-values 16 s + 8 h + 0..7.
+__device__ __forceinline__ u16x8 lk_row(const uint16_t* tile, int row, int s, int h) {
+  return *reinterpret_cast<const u16x8*>(tile + row * LK_K + (((2 * s + h) ^ lk_swz(row)) << 3));
+}
+
+// Column operand: column c0 + (lane & 31) of a [64][COLS] tile, the same k-values (its rows).
+template <int COLS>
+__device__ __forceinline__ u16x8 lk_col(const uint16_t* tile, int c0, int s, int lane) {
+  const int i = lane & 15, ch = (c0 >> 3) + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+  const int row = 16 * s + 8 * (lane >> 5) + (i >> 2);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lk_tr_t)(tile + row * COLS + ((ch ^ lk_swz(row)) << 3) + ((i & 1) << 2)));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lk_tr_t)(tile + (row + 4) * COLS + ((ch ^ lk_swz(row + 4)) << 3) + ((i & 1) << 2)));
+  const s16x4 both[2] = {lo, hi};
+  u16x8 r;
+  __builtin_memcpy(&r, both, 16);
+  return r;
+}
+
+// Copies a [rows R0 ..][64 k] or (COL) [64 k][columns C0 ..] tile by DMA; what lies outside
+// (`rend` rows, `kend` k-values; COL: `rend` columns) is read as zeros.  SIDE rows or columns.
+template <int SIDE, int NW, bool COL>
+struct LkStage {
+  static constexpr int CPR = COL ? SIDE / 8 : LK_K / 8;  // chunks a tile row
+  static constexpr int N = SIDE * LK_K / 512 / NW;       // DMA instructions a wave
+  static_assert(SIDE * LK_K % (512 * NW) == 0, "whole instructions a wave");
+  const uint16_t* base[N];
+  int k[N], ld;
+  bool in[N];
+  __device__ __forceinline__ void init(const uint16_t* src, int ld_, int r0, int rend, int wave, int lane) {
+    ld = ld_;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int q = (wave + NW * i) * 64 + lane, row = q / CPR, c = (q % CPR) ^ lk_swz(row);
+      const int side = COL ? r0 + 8 * c : r0 + row;
+      k[i] = COL ? row : 8 * c;
+      in[i] = side < rend;
+      base[i] = src + (COL ? (size_t)row * ld + side : (size_t)side * ld + k[i]);
+    }
+  }
+  __device__ __forceinline__ void issue(uint16_t* dst, int k0, int kend, int wave) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint16_t* p = base[i] + (COL ? (size_t)k0 * ld : (size_t)k0);
+      if (!in[i] || k0 + k[i] >= kend) p = reinterpret_cast<const uint16_t*>(&lk_zero);
+      __builtin_amdgcn_global_load_lds((const void*)p, (lk_lds_t)(dst + (wave + NW * i) * 512), 16, 0, 0);
+    }
+  }
+};
+
+// MODE 0 / 1: lane side = hidden rows, register side = vocabulary rows, k = H.
+// MODE 2: lane = the piece's vocabulary rows, register = H, k = hidden rows.
+// MODE 3: lane = hidden rows, register = H, k = a split of the piece.
+template <bool BF, int MODE, int BL, int BR, int WL, int WR>
+__global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
+  constexpr int NW = WL * WR, TL = BL / WL, TR = BR / WR, FL = TL / 32, FR = TR / 32;
+  constexpr bool LCOL = MODE == 2, RCOL = MODE >= 2;
+  constexpr int STAGE = (BL + BR) * LK_K;
+  static_assert(2 * STAGE * 2 <= 160 * 1024 && BL % (32 * WL) == 0 && BR % (32 * WR) == 0, "tile");
+  __shared__ __attribute__((aligned(16))) uint16_t sm[2 * STAGE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int wl = wave / WR, wr = wave % WR;
+  const int cnt = a.cnt[0];
+  const int nl = (MODE == 2 ? a.vn : a.Mp) / BL;
+  const int nr = MODE >= 2 ? (a.H + BR - 1) / BR : a.vn / BR;
+  // blocks go round the 8 XCDs: each gets a run of tiles, walked in bands of 8 lane-side
+  // tiles, so that what an XCD has in flight shares its L2
+  int t, z = 0;
+  {
+    const int T = nl * nr * (MODE == 3 ? a.splits : 1), x = blockIdx.x & 7, q = T >> 3, r = T & 7;
+    t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
+  }
+  if constexpr (MODE == 3) {
+    z = t / (nl * nr);
+    t -= z * nl * nr;
+  }
+  const int band = t / (8 * nr), bl = t - band * 8 * nr, bw = min(8, nl - 8 * band);
+  const int l0 = (8 * band + bl % bw) * BL, r0 = (bl / bw) * BR;
+  if (MODE != 2 && l0 >= cnt) return;
+  int kb = 0, ke = a.Hp;
+  if constexpr (MODE == 2) ke = (cnt + LK_K - 1) / LK_K * LK_K;
+  if constexpr (MODE == 3) {
+    const int per = (a.vn / LK_K + a.splits - 1) / a.splits * LK_K;
+    kb = min(a.vn, z * per);
+    ke = min(a.vn, kb + per);
+  }
+  LkStage<BL, NW, LCOL> sl;
+  LkStage<BR, NW, RCOL> sr;
+  if constexpr (MODE <= 1) {
+    sl.init(a.hc, a.Hp, l0, a.Mp, wave, lane);
+    sr.init(a.table, a.H, a.v0 + r0, a.V, wave, lane);
+  } else if constexpr (MODE == 2) {
+    sl.init(a.d, a.ldd, l0, a.vn, wave, lane);
+    sr.init(a.hc, a.Hp, r0, a.Hp, wave, lane);
+  } else {
+    sl.init(a.d, a.ldd, l0, a.Mp, wave, lane);
+    sr.init(a.table + (size_t)a.v0 * a.H, a.H, r0, a.H, wave, lane);
+  }
+  const int kl = MODE == 3 ? a.vn : MODE == 2 ? a.Mp : a.Hp;                  // k-values that exist
+  const int kr = MODE == 3 ? min(a.vn, a.V - a.v0) : MODE == 2 ? a.Mp : a.H;
+  auto stage = [&](int k0, int buf) {
+    sl.issue(sm + buf * STAGE, k0, kl, wave);
+    sr.issue(sm + buf * STAGE + BL * LK_K, k0, kr, wave);
+  };
+  f32x16 acc[FR][FL];
+#pragma unroll
+  for (int i = 0; i < FR; ++i)
+#pragma unroll
+    for (int j = 0; j < FL; ++j) acc[i][j] = (f32x16)0.f;
+  if (kb < ke) stage(kb, 0);
+  int buf = 0;
+  for (int k0 = kb; k0 < ke; k0 += LK_K, buf ^= 1) {
+    // this wave's copies have landed and its reads of the other buffer are done; every wave's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (k0 + LK_K < ke) stage(k0 + LK_K, buf ^ 1);
+    const uint16_t *ls = sm + buf * STAGE, *rs = ls + BL * LK_K;
+#pragma unroll
+    for (int s = 0; s < LK_K / 16; ++s) {
+      u16x8 lf[FL], rf[FR];
+#pragma unroll
+      for (int j = 0; j < FL; ++j)
+        lf[j] = LCOL ? lk_col<BL>(ls, wl * TL + 32 * j, s, lane) : lk_row(ls, wl * TL + 32 * j + (lane & 31), s, h);
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+        rf[i] = RCOL ? lk_col<BR>(rs, wr * TR + 32 * i, s, lane) : lk_row(rs, wr * TR + 32 * i + (lane & 31), s, h);
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FL; ++j) acc[i][j] = lk_mma<BF>(rf[i], lf[j], acc[i][j]);
+    }
+  }
+  // register r of acc[i][j]: register-side index r0 + wr TR + 32 i + 8 (r >> 2) + 4 h + (r & 3)
+  const int ln = l0 + wl * TL + (lane & 31), rn = r0 + wr * TR + 4 * h;
+  if constexpr (MODE == 0) {
+    float2* red = reinterpret_cast<float2*>(sm);  // [WR][BL]
+    __syncthreads();
+    const int vend = a.V - a.v0;
+#pragma unroll
+    for (int j = 0; j < FL; ++j) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (r0 + BR > vend && rn + 32 * i + 8 * (r >> 2) + (r & 3) >= vend) acc[i][j][r] = -INFINITY;
+          top = fmaxf(top, acc[i][j][r]);
+        }
+      top = lk_max_halves(top);
+      // z - top first: a loss near 0 is a difference of large logits
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += lk_exp(acc[i][j][r] - ref);
+      sum = lk_sum_halves(sum);
+      if (h == 0) red[wr * BL + wl * TL + 32 * j + lane] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < BL; n += NW * 64) {
+      float2 x = red[n];
+#pragma unroll
+      for (int w = 1; w < WR; ++w) {
+        const float2 y = red[w * BL + n];
+        const float m = fmaxf(x.x, y.x), ref = m == -INFINITY ? 0.f : m;
+        x = make_float2(m, x.y * lk_exp(x.x - ref) + y.y * lk_exp(y.x - ref));
+      }
+      a.part[(size_t)(r0 / BR) * a.Mp + l0 + n] = x;
+    }
+  } else if constexpr (MODE == 1) {
+    const int vend = a.V - a.v0;
+#pragma unroll
+    for (int j = 0; j < FL; ++j) {
+      const int n = ln + 32 * j;
+      const float lse = n < cnt ? a.lse[n] : INFINITY;
+      const float w = (a.w != nullptr && n < cnt ? a.w[n] : 1.f) * (BF ? 1.f : LK_FP16);
+      const int y = (n < cnt ? a.lab[n] : -1) - a.v0 - rn;  // its place in this lane's registers
+      const bool here = y >= 0 && y < TR;
+      uint16_t* row = a.d + (size_t)n * a.ldd + rn;
+#pragma unroll
+      for (int i = 0; i < FR; ++i) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LK_LOG2E, -lse));
+        if (__any(here)) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (y == 32 * i + 8 * (r >> 2) + (r & 3)) acc[i][j][r] -= 1.f;
+        }
+        if (r0 + BR > vend) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (rn + 32 * i + 8 * (r >> 2) + (r & 3) >= vend) acc[i][j][r] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint2*>(row + 32 * i + 8 * e) =
+              lk_pack4<BF>(acc[i][j][4 * e] * w, acc[i][j][4 * e + 1] * w, acc[i][j][4 * e + 2] * w,
+                           acc[i][j][4 * e + 3] * w);
+      }
+    }
+  } else {
+    const float f = MODE == 3 ? 1.f
+                              : (a.mode == 2 ? a.gmax[0] : a.mode == 1 ? a.g[0] : a.g[0] / (float)max(cnt, 1)) *
+                                    (BF ? 1.f : 1.f / LK_FP16);
+#pragma unroll
+    for (int j = 0; j < FL; ++j) {
+      const int n = ln + 32 * j;
+      if (MODE == 2 && a.v0 + n >= a.V) continue;
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = rn + 32 * i + 8 * e;
+          if (c >= a.H) continue;
+          if constexpr (MODE == 2) {
+            *reinterpret_cast<uint2*>(a.dtable + (size_t)(a.v0 + n) * a.H + c) =
+                lk_pack4<BF>(acc[i][j][4 * e] * f, acc[i][j][4 * e + 1] * f, acc[i][j][4 * e + 2] * f,
+                             acc[i][j][4 * e + 3] * f);
+          } else {
+            float4* p = reinterpret_cast<float4*>(a.share + ((size_t)z * a.Mp + n) * a.Hp + c);
+            float4 x = make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
+            if (!a.first) {
+              const float4 y = *p;
+              x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+            }
+            *p = x;
+          }
+        }
+    }
+  }
+}
+
+// ---- joins -----------------------------------------------------------------------------
+// 64 rows a block: L from the tiles' (maximum, sum), the label's logit, the loss.
+template <bool BF>
+__global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
+  __shared__ float2 red[4][64];
+  __shared__ float zy[64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m0 = blockIdx.x * 64, cnt = a.cnt[0];
+  if (m0 >= cnt) return;
+  const int m = m0 + lane;
+  float2 x = make_float2(-INFINITY, 0.f);
+  for (int t = wave; t < tiles; t += 32) {
+    float2 y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      y[k] = make_float2(-INFINITY, 0.f);
+      if (t + 4 * k < tiles) y[k] = a.part[(size_t)(t + 4 * k) * a.Mp + m];
+    }
+    float top = x.x;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, y[k].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float s = x.y * lk_exp(x.x - ref);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += y[k].y * lk_exp(y[k].x - ref);
+    x = make_float2(top, s);
+  }
+  red[wave][lane] = x;
+  for (int i = wave; i < 64; i += 4) {  // z[y]: a wave a row
+    const int y = m0 + i < cnt ? a.lab[m0 + i] : -1;
+    float s = 0.f;
+    if (y >= 0) {
+      const u16x8* hr = reinterpret_cast<const u16x8*>(a.hc + (size_t)(m0 + i) * a.Hp);
+      const u16x8* er = reinterpret_cast<const u16x8*>(a.table + (size_t)y * a.H);
+      for (int c = lane; c < a.H / 8; c += 64) {
+        const u16x8 p = hr[c], q = er[c];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s = fmaf(lk_float<BF>(p[k]), lk_float<BF>(q[k]), s);
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) zy[i] = s;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  float top = fmaxf(fmaxf(red[0][lane].x, red[1][lane].x), fmaxf(red[2][lane].x, red[3][lane].x));
+  const float ref = top == -INFINITY ? 0.f : top;
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) s += red[w][lane].y * lk_exp(red[w][lane].x - ref);
+  float ls = __logf(s);
+  if (m < cnt) {
+    if (a.lab[m] == -2) ls = __builtin_nanf("");
+    const float loss = (top - zy[lane]) + ls;
+    a.lse[m] = (top + ls) * LK_LOG2E;
+    a.rl[m] = loss;
+    if (a.mode == 2) a.loss[a.rows[m]] = loss;
+  }
+}
+
+__device__ __forceinline__ float lk_block_sum(float s, float* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  s = 0.f;
+  for (int w = 0; w < 16; ++w) s += red[w];
+  return s;
+}
+
+// mean (no labelled row: 0 / 0, as the mean of nothing) or sum
+__global__ void __launch_bounds__(1024) loss_sum_kernel(LossArgs a) {
+  __shared__ float red[16];
+  const int cnt = a.cnt[0];
+  float s = 0.f;
+  for (int m = threadIdx.x; m < cnt; m += 1024) s += a.rl[m];
+  s = lk_block_sum(s, red);
+  if (threadIdx.x == 0) a.loss[0] = a.mode == 0 ? s / (float)cnt : s;
+}
+
+// none: w = g / max |g| (in [-1, 1]), gmax
+__global__ void __launch_bounds__(1024) loss_weights_kernel(LossArgs a, float* gmax) {
+  __shared__ float red[16];
+  const int cnt = a.cnt[0], lane = threadIdx.x & 63;
+  float t = 0.f;
+  for (int m = threadIdx.x; m < cnt; m += 1024) t = fmaxf(t, fabsf(a.g[a.rows[m]]));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
+  if (lane == 0) red[threadIdx.x >> 6] = t;
+  __syncthreads();
+  for (int w = 0; w < 16; ++w) t = fmaxf(t, red[w]);
+  for (int m = threadIdx.x; m < cnt; m += 1024) {
+    const float g = a.g[a.rows[m]];
+    a.w[m] = t > 0.f ? g / t : g;
+  }
+  if (threadIdx.x == 0) gmax[0] = t;
+}
+
+// dh: the shares' sum, in order, for labelled rows; zeros for the others.  4 columns a thread.
+template <bool BF>
+__global__ void __launch_bounds__(256) loss_dh_kernel(LossArgs a) {
+  const int nch = a.H / 4;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long)a.N * nch) return;
+  const int row = (int)(i / nch), c = (int)(i - (long)row * nch) * 4, m = a.pos[row];
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (m >= 0) {
+    for (int z = 0; z < a.splits; ++z) {
+      const float4 x = *reinterpret_cast<const float4*>(a.share + ((size_t)z * a.Mp + m) * a.Hp + c);
+      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    }
+    const float f = (a.mode == 2 ? a.gmax[0] : a.mode == 1 ? a.g[0] : a.g[0] / (float)a.cnt[0]) *
+                    (BF ? 1.f : 1.f / LK_FP16);
+    s.x *= f, s.y *= f, s.z *= f, s.w *= f;
+  }
+  *reinterpret_cast<uint2*>(a.dh + (size_t)row * a.H + c) = lk_pack4<BF>(s.x, s.y, s.z, s.w);
+}
+
+// ---- plan ------------------------------------------------------------------------------
+// Big tiles (256 x 256, 8 waves) read 3 KB of LDS per 4 products; a few hundred rows leave
+// most of the card without one, so there 64 x 64 tiles of 4 waves run instead.
+struct LossPlan {
+  int Mp, Hp, small, vtiles, piece, splits;
+};
+
+constexpr long LK_PIECE = 1L << 27;  // elements of d (256 MB: what the last-level cache holds)
+
+LossPlan lk_plan(int N, int V, int H) {
+  LossPlan p;
+  p.Mp = (N + LK_PAD - 1) / LK_PAD * LK_PAD;
+  p.Hp = (H + LK_K - 1) / LK_K * LK_K;
+  const long vp = ((long)V + LK_PAD - 1) / LK_PAD * LK_PAD;
+  p.small = (p.Mp / 256) * (vp / 256) < 256;
+  p.vtiles = (int)(vp / (p.small ? 64 : 256));
+  long piece = LK_PIECE / p.Mp / LK_PAD * LK_PAD;
+  if (piece < 4 * LK_PAD) piece = 4 * LK_PAD;
+  p.piece = (int)(piece < vp ? piece : vp);
+  // dh: blocks over the card, each with at least 4 steps of k
+  const int bl = p.small ? 64 : 256, br = p.small ? 64 : 192;
+  const int tiles = p.Mp / bl * ((H + br - 1) / br);
+  int s = (512 + tiles - 1) / tiles;
+  const int most = p.piece / (4 * LK_K);
+  p.splits = s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s;
+  if (p.splits > 64) p.splits = 64;
+  return p;
+}
+
+template <bool BF, int MODE>
+void lk_gemm(const LossArgs& a, const LossPlan& p, hipStream_t st) {
+  if (p.small) {
+    const int nl = (MODE == 2 ? a.vn : a.Mp) / 64, nr = MODE >= 2 ? (a.H + 63) / 64 : a.vn / 64;
+    loss_gemm_kernel<BF, MODE, 64, 64, 2, 2>
+        <<<dim3(nl * nr * (MODE == 3 ? a.splits : 1)), dim3(256), 0, st>>>(a);
+  } else if constexpr (MODE <= 1) {
+    loss_gemm_kernel<BF, MODE, 256, 256, 2, 4><<<dim3(a.Mp / 256 * (a.vn / 256)), dim3(512), 0, st>>>(a);
+  } else {
+    const int nl = (MODE == 2 ? a.vn : a.Mp) / 256, nr = (a.H + 191) / 192;
+    loss_gemm_kernel<BF, MODE, 256, 192, 4, 2>
+        <<<dim3(nl * nr * (MODE == 3 ? a.splits : 1)), dim3(512), 0, st>>>(a);
+  }
+}
+
+template <bool BF>
+void lk_forward(LossArgs a, const LossPlan& p, hipStream_t st) {
+  loss_rows_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
+  loss_gather_kernel<<<dim3((unsigned)(((long)p.Mp * (p.Hp / 8) + 255) / 256)), dim3(256), 0, st>>>(a);
+  a.v0 = 0;
+  a.vn = p.vtiles * (p.small ? 64 : 256);
+  lk_gemm<BF, 0>(a, p, st);
+  loss_join_kernel<BF><<<dim3(p.Mp / 64), dim3(256), 0, st>>>(a, p.vtiles);
+  if (a.mode != 2) loss_sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
+}
+
+template <bool BF>
+void lk_backward(LossArgs a, const LossPlan& p, hipStream_t st) {
+  if (a.mode == 2) loss_weights_kernel<<<dim3(1), dim3(1024), 0, st>>>(a, const_cast<float*>(a.gmax));
+  a.ldd = p.piece;
+  a.splits = p.splits;
+  const int vp = p.vtiles * (p.small ? 64 : 256);
+  for (int v0 = 0; v0 < vp; v0 += p.piece) {
+    a.v0 = v0;
+    a.vn = vp - v0 < p.piece ? vp - v0 : p.piece;
+    a.first = v0 == 0;
+    lk_gemm<BF, 1>(a, p, st);
+    if (a.dtable != nullptr) lk_gemm<BF, 2>(a, p, st);
+    if (a.dh != nullptr) lk_gemm<BF, 3>(a, p, st);
+  }
+  if (a.dh != nullptr)
+    loss_dh_kernel<BF><<<dim3((unsigned)(((long)a.N * (a.H / 4) + 255) / 256)), dim3(256), 0, st>>>(a);
+}
+
+bool lk_bad(int N, int V, int H, int mode) {
+  return N <= 0 || N > (1 << 24) || V <= 0 || V > (1 << 24) || H <= 0 || H % 8 != 0 || H > (1 << 14) || mode < 0 ||
+         mode > 2 || ((long)N + 255) / 64 * (((long)V + 255) / 64) > 0x7fffffffL;
+}
+
+// state: ints pos[N], rows[Mp], lab[Mp], cnt[64]; floats lse[Mp], rl[Mp]
+void lk_state(LossArgs& a, const LossPlan& p, void* state) {
+  int* s = (int*)state;
+  a.cnt = s;
+  a.rows = s + 64;
+  a.lab = a.rows + p.Mp;
+  a.lse = (float*)(a.lab + p.Mp);
+  a.rl = a.lse + p.Mp;
+  a.pos = (int*)(a.rl + p.Mp);
+  a.Mp = p.Mp, a.Hp = p.Hp;
+}
+
+}  // namespace
+
+extern "C" {
+
+// out[0..5]: rows and columns of hc; 32-bit words of state, of the forward's and of the
+// backward's workspace (in units of 64 words); elements of d are part of the last
+int sg_loss_plan(int N, int V, int H, void* out) {
+  if (lk_bad(N, V, H, 0)) return 1;
+  const LossPlan p = lk_plan(N, V, H);
+  int* o = (int*)out;
+  o[0] = p.Mp;
+  o[1] = p.Hp;
+  o[2] = (64 + 4 * p.Mp + N + 63) / 64;
+  o[3] = (int)((2L * p.vtiles * p.Mp + 63) / 64);
+  o[4] = (int)((64 + p.Mp + (long)p.Mp * p.piece / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
+  return 0;
+}
+
+// mode: 0 mean, 1 sum (loss [1]), 2 none (loss [N])
+int sg_loss_fwd(const void* h, const void* table, const void* labels, int is64, int ignore, void* hc, void* state,
+                void* ws, void* loss, int N, int V, int H, int mode, int fp16, hipStream_t st) {
+  if (lk_bad(N, V, H, mode)) return 1;
+  const LossPlan p = lk_plan(N, V, H);
+  LossArgs a = {};
+  a.h = (const uint16_t*)h, a.table = (const uint16_t*)table, a.labels = labels, a.is64 = is64, a.ignore = ignore;
+  a.hc = (uint16_t*)hc, a.loss = (float*)loss, a.part = (float2*)ws;
+  a.N = N, a.V = V, a.H = H, a.mode = mode;
+  lk_state(a, p, state);
+  fp16 ? lk_forward<false>(a, p, st) : lk_forward<true>(a, p, st);
+  return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+
+// g: the gradient of loss ([1], none: [N]); dh or dtable may be null (not wanted)
+int sg_loss_bwd(const void* hc, const void* table, void* state, const void* g, void* ws, void* dh, void* dtable, int N,
+                int V, int H, int mode, int fp16, hipStream_t st) {
+  if (lk_bad(N, V, H, mode)) return 1;
+  const LossPlan p = lk_plan(N, V, H);
+  LossArgs a = {};
+  a.hc = (uint16_t*)const_cast<void*>(hc), a.table = (const uint16_t*)table, a.g = (const float*)g;
+  a.dh = (uint16_t*)dh, a.dtable = (uint16_t*)dtable;
+  a.N = N, a.V = V, a.H = H, a.mode = mode;
+  lk_state(a, p, state);
+  float* w = (float*)ws;
+  a.gmax = w;
+  a.w = mode == 2 ? w + 64 : nullptr;
+  a.d = (uint16_t*)(w + 64 + p.Mp);
+  a.share = w + 64 + p.Mp + (size_t)p.Mp * p.piece / 2;
+  fp16 ? lk_backward<false>(a, p, st) : lk_backward<true>(a, p, st);
+  return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+
+}  // extern "C"

@@ -56,3 +56,21 @@ def test_tiled_attention_refuses_mismatched_operands():
             train_ops.tiled_attention(*bad)
     with pytest.raises(TypeError, match="tiled_attention"):
         train_ops.tiled_attention(q, k.half(), v)
+
+
+@pytest.mark.parametrize("h,table,labels,kw,err", [
+    (torch.zeros(3, 16), torch.zeros(4, 16), _ids(3), {}, TypeError),                       # fp32
+    (torch.zeros(3, 16).half(), torch.zeros(4, 16).bfloat16(), _ids(3), {}, TypeError),     # two types
+    (torch.zeros(3, 16).half(), torch.zeros(4, 16).half(), torch.zeros(3), {}, TypeError),  # labels are whole numbers
+    (torch.zeros(3, 16).half(), torch.zeros(4, 16).half(), _ids(4), {}, ValueError),
+    (torch.zeros(3, 16).half(), torch.zeros(4, 24).half(), _ids(3), {}, ValueError),
+    (torch.zeros(3, 12).half(), torch.zeros(4, 12).half(), _ids(3), {}, ValueError),        # rows of no whole 16 bytes
+    (torch.zeros(0, 16).half(), torch.zeros(4, 16).half(), _ids(0), {}, ValueError),
+    (torch.zeros(3, 16).half(), torch.zeros(0, 16).half(), _ids(3), {}, ValueError),
+    (torch.zeros(3, 16).half(), torch.zeros(4, 16).half(), _ids(3), dict(reduction="max"), ValueError),
+    (torch.zeros(3, 16).half(), torch.zeros(4, 16).half(), _ids(3), dict(ignore_index=1 << 40), ValueError),
+    (torch.zeros(3, 16).half(), torch.zeros(4, 16).half(), _ids(3), {}, ValueError),        # not on a GPU
+])
+def test_lm_loss_refuses(h, table, labels, kw, err):
+    with pytest.raises(err, match="lm_loss"):
+        train_ops.lm_loss(h, table, labels, **kw)
