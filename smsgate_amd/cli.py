@@ -240,7 +240,7 @@ def train_config(a, world: int = 1):
     return recipe(a.model, a.steps, a.batch, world=world, lr=a.lr, n_examples=a.examples, seed=a.seed,
                   ckpt_dir=a.ckpt_dir, ckpt_every=a.ckpt_every, resume=a.resume, bucket_mb=a.bucket_mb,
                   answer_format=a.answer_format, families=None if a.families == "legacy" else a.families,
-                  negatives=a.negatives)
+                  negatives=a.negatives, hip_ops=a.hip_ops)
 
 
 def _train(a, settings) -> None:
@@ -386,6 +386,9 @@ def build_parser() -> argparse.ArgumentParser:
                          "per copied field; copy: the body's tokens (the checkpoint records it; the engine follows)")
     tr.add_argument("--negatives", type=float, default=R.negatives,
                     help="share of non-transaction examples (txn_type unknown / otp, null fields)")
+    tr.add_argument("--hip-ops", action="store_true", default=R.hip_ops,
+                    help="embedding, attention and the copy / span loss by this package's own kernels "
+                         "(models/train_ops.py) instead of torch's")
     tr.add_argument("--families", default="train", help="train (every training SMS layout) | legacy (the two "
                     "reference formats only)")
     sp.add_parser("config")

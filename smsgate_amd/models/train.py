@@ -90,6 +90,11 @@ class TrainConfig:
     # fused HIP RMSNorm / RoPE / SwiGLU forward+backward (models/train_ops.py) on the GPU;
     # False: reference_forward (plain PyTorch elementwise chains)
     fused: bool = True
+    # the embedding, the attention and the copy / span formats' loss by this package's own
+    # kernels too (models/train_ops.py embed_lookup, tiled_attention, lm_loss) instead of
+    # F.embedding, SDPA and a matrix of logits: the same mathematics with other roundings, so
+    # another run of the same recipe; needs a GPU and ``fused``
+    hip_ops: bool = False
     eval_every: int = 0  # call on_eval(step, serving weights) every N steps (0 = never)
     # "copy": every copied value written with the body's own tokens; "span": as two
     # pointers to its first and last body token (serving/fsm.py build_span_fsm)
@@ -360,6 +365,14 @@ def qa_batch(prefix: List[int], exs, pad: int, device, lay):
     return out[0], out[1], out[2], tuple(out[3:])
 
 
+def _answer_loss(h: torch.Tensor, table: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
+    """Mean next-token cross-entropy of the labelled rows (copy / span formats)."""
+    sel = labels.view(-1) >= 0
+    hs = h.reshape(-1, h.shape[-1])[sel]
+    logits = hs @ table.t()
+    return F.cross_entropy(logits.float(), labels.view(-1)[sel])
+
+
 def latest_checkpoint(ckpt_dir: Optional[str]) -> Optional[Path]:
     if not ckpt_dir or not os.path.isdir(ckpt_dir):
         return None
@@ -409,6 +422,10 @@ def train_extractor(cfg: TrainConfig, device="cuda", log: Callable[[str], None] 
 
     from ..parallel.ddp import GradBuckets
 
+    from . import train_ops
+
+    if cfg.hip_ops and not (cfg.fused and train_ops.available(device)):
+        raise ValueError("train_extractor: hip_ops needs a GPU and the fused forward")
     ddp = dist.is_initialized() and cfg.data_parallel
     rank = dist.get_rank() if ddp else 0
     world = dist.get_world_size() if ddp else 1
@@ -475,12 +492,12 @@ def train_extractor(cfg: TrainConfig, device="cuda", log: Callable[[str], None] 
             if rank == 0:
                 rng.setstate(_as_rng_state(state["rng"]))
         log(f"train: resumed from {ck} at step {start}")
-    from . import train_ops
-
     if cfg.fused and train_ops.available(device):
-        forward = train_ops.fused_forward
+        def forward(w_, ids_, add_, lengths=None):
+            return train_ops.fused_forward(w_, ids_, add_, hip_ops=cfg.hip_ops,
+                                           lengths=lengths if cfg.hip_ops else None)
     else:
-        def forward(w_, ids_, add_):
+        def forward(w_, ids_, add_, lengths=None):
             return reference_forward(w_, ids_, compute_dtype=torch.float32, return_hidden=True, add_ids=add_)
     t0 = time.perf_counter()
     for step in range(start, cfg.steps):
@@ -496,7 +513,8 @@ def train_extractor(cfg: TrainConfig, device="cuda", log: Callable[[str], None] 
                 from ..serving.qa import qa_logits, qa_loss
 
                 ids, add, qpos, targets = qa_batch(prefix, exs, tok.pad, device, fsm.lay)
-                h = forward(w, ids, add)
+                # a row ends with its last query
+                h = forward(w, ids, add, (qpos[:, -1] + 1).int() if cfg.hip_ops else None)
                 # decisions of the (global) batch: class + a start per field + an end per
                 # non-null field -- counted on the host, divided over the ranks
                 n_dec = sum(1 + len(sp) + sum(1 for s_, _ in sp if s_ >= 0) for _, (_, sp) in exs_g)
@@ -505,10 +523,10 @@ def train_extractor(cfg: TrainConfig, device="cuda", log: Callable[[str], None] 
             else:
                 ids, labels, add = _batch(prefix, exs, tok.pad, device, fsm.ptr0)
                 h = forward(w, ids, add)
-                sel = labels.view(-1) >= 0
-                hs = h.reshape(-1, h.shape[-1])[sel]
-                logits = hs @ w.embed[:v_dec].t()
-                loss = F.cross_entropy(logits.float(), labels.view(-1)[sel])
+                if cfg.hip_ops:  # the unlabelled rows are left out on the GPU
+                    loss = train_ops.lm_loss(h, w.embed[:v_dec].to(h.dtype), labels)
+                else:
+                    loss = _answer_loss(h, w.embed[:v_dec], labels)
         if gb is not None:
             gb.zero_grad()
             loss.backward()  # bucket all-reduces start as gradients land

@@ -21,6 +21,15 @@ autograd Function with a hand-written backward:
   56 ms of a step against SDPA's ~6 (``r05_train_step_sdpa_ab.jsonl``), so SDPA (flash)
   stays the default.
 
+Three operators of the whole step, on request (``hip_ops``; TrainConfig.hip_ops):
+
+* :func:`embed_lookup`: both embedding rows of a position in one pass, the table's gradient
+  by sorted ids in a fixed order (csrc/embed_kernels.hip);
+* :func:`tiled_attention`: attention of any length in matrix instructions, its backward pass
+  recomputing the probabilities (csrc/attn_grad_kernels.hip);
+* :func:`lm_loss`: cross entropy over the embedding's rows without logits, for the copy and
+  span answer formats (csrc/loss_kernels.hip).
+
 GEMMs stay hipBLASLt (autocast bf16), so the math is
 reference_forward's up to bf16 rounding order (tests/test_train_ops_gpu.py compares
 losses and gradients).  CPU / no-library: reference_forward.
@@ -29,6 +38,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 import os
 from typing import Optional
@@ -442,16 +452,25 @@ def swiglu(gu: torch.Tensor) -> torch.Tensor:
     return _SwiGLU.apply(gu)
 
 
-def fused_forward(w: ExtractorWeights, ids: torch.Tensor, add_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+def fused_forward(w: ExtractorWeights, ids: torch.Tensor, add_ids: Optional[torch.Tensor] = None, *,
+                  hip_ops: bool = False, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Final-normed hidden states [B, T, H] (bf16) of ``reference_forward(w, ids,
     return_hidden=True, add_ids=add_ids)``; call under ``torch.autocast(bf16)`` with fp32
-    master weights (models/train.py)."""
+    master weights (models/train.py).  ``hip_ops``: the embedding is :func:`embed_lookup` and
+    the attention :func:`tiled_attention` (over the first ``lengths[b]`` positions of each
+    row, int32; the states behind them are then not meant to be read) instead of
+    F.embedding and SDPA."""
     cfg = w.cfg
     B, T = ids.shape
     nh, nkv, D = cfg.heads, cfg.kv_heads, cfg.head_dim
-    x = F.embedding(ids, w.embed)
-    if add_ids is not None:
-        x = x + F.embedding(add_ids.clamp(min=0), w.embed) * (add_ids >= 0).unsqueeze(-1).to(x.dtype)
+    if hip_ops:
+        x = embed_lookup(ids, w.embed, add_ids)
+    else:
+        if lengths is not None:
+            raise ValueError("fused_forward: lengths need hip_ops")
+        x = F.embedding(ids, w.embed)
+        if add_ids is not None:
+            x = x + F.embedding(add_ids.clamp(min=0), w.embed) * (add_ids >= 0).unsqueeze(-1).to(x.dtype)
     x = x.float().contiguous()
     cos, sin = _rope_tables(T, D, cfg.rope_theta, ids.device)
     cos, sin = cos.reshape(T, D // 2).contiguous(), sin.reshape(T, D // 2).contiguous()
@@ -463,6 +482,10 @@ def fused_forward(w: ExtractorWeights, ids: torch.Tensor, add_ids: Optional[torc
     sdpa = os.environ.get("SMSGATE_TRAIN_SDPA", "")
     rep = nh // nkv if sdpa == "efficient" else 1
     own = sdpa == "own" and T <= ATTN_MAX_T
+    if hip_ops:
+        rep, own = 1, functools.partial(tiled_attention, lengths=lengths)
+    else:
+        own = attention if own else None
     with _sdpa_backend():
         for i in range(cfg.layers):
             x = _layer(w, i, x, cos, sin, scale, B, T, nh, nkv, D, rep, own)
@@ -481,13 +504,14 @@ def _sdpa_backend():
                         "math": SDPBackend.MATH}[name])
 
 
-def _layer(w, i, x, cos, sin, scale, B, T, nh, nkv, D, rep=1, own=False):
-    """One decoder layer of the residual stream ``x`` (fp32)."""
+def _layer(w, i, x, cos, sin, scale, B, T, nh, nkv, D, rep=1, own=None):
+    """One decoder layer of the residual stream ``x`` (fp32); ``own``: an attention of
+    (q, k, v, scale) in SDPA's place."""
     eps = w.cfg.eps
     h = rms_norm(x, w.ln1[i], eps)
     q, k, v = rope_split(h @ w.qkv[i].t(), cos, sin, nh, nkv, rep)
-    if own:
-        a = attention(q, k, v, scale)
+    if own is not None:
+        a = own(q, k, v, scale)
     else:
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scale,
                                            enable_gqa=nh != nkv * rep).transpose(1, 2).reshape(B, T, nh * D)

@@ -74,3 +74,17 @@ def test_tiled_attention_refuses_mismatched_operands():
 def test_lm_loss_refuses(h, table, labels, kw, err):
     with pytest.raises(err, match="lm_loss"):
         train_ops.lm_loss(h, table, labels, **kw)
+
+
+def test_hip_ops_is_a_training_option_that_needs_a_gpu():
+    from smsgate_amd.cli import build_parser, train_config
+    from smsgate_amd.models.train import FLAGSHIP_RECIPE, TrainConfig, train_extractor
+
+    assert not FLAGSHIP_RECIPE.hip_ops
+    args = ["train-extractor", "--out", "x.safetensors"]
+    assert not train_config(build_parser().parse_args(args)).hip_ops
+    assert train_config(build_parser().parse_args(args + ["--hip-ops"])).hip_ops
+    with pytest.raises(ValueError, match="hip_ops"):
+        train_extractor(TrainConfig(model="tiny", steps=1, n_examples=2, hip_ops=True), device="cpu")
+    with pytest.raises(ValueError, match="hip_ops"):
+        train_extractor(TrainConfig(model="tiny", steps=1, n_examples=2, hip_ops=True, fused=False), device="cuda")
