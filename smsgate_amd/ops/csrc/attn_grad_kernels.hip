@@ -27,8 +27,8 @@
 //             dV^T = dO^T P,  dK^T = Q^T dS
 // The operand of the wave's own 32 rows stays in registers; the tiles that are walked are
 // copied into LDS by the DMA path (global_load_lds), two buffers, one barrier a tile.  A
-// tile's 16-byte chunks are XORed with a bijection of row & 7 that spreads both the row
-// reads (8 rows, one chunk) and the transposing reads (4 rows, 2 chunks) over all banks.
+// tile's 16-byte chunks are XORed by row, so that neither row nor transposing reads meet on
+// a bank.
 //
 // Sums, L, D and the running maximum are fp32.  The forward keeps what rounding took from o
 // (another value of the type), so that D is taken from 16 more bits of o: from the rounded o
@@ -106,7 +106,16 @@ __device__ __forceinline__ float at_sum_halves(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-__device__ __forceinline__ int at_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+// What is XORed into the 16-byte chunk index of row `row` of a tile.  LDS serves 256 bytes a
+// cycle over 64 banks: 16 lanes of a row read (16 rows, one chunk) or 32 of a transposing
+// read (4 rows, 4 chunks); either way the chunks differ modulo 256 bytes.
+template <int D>
+__device__ __forceinline__ int at_swz(int row) {
+  if constexpr (D == 64)  // 128-byte rows: row & 1 is half of the banks already
+    return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) | ((row >> 3) & 1) << 1;
+  else
+    return (row & 3) << 2 | ((row >> 2) & 3);
+}
 
 // Rows [r0, r0 + ROWS) of a [.., D] matrix into LDS, rows at or behind `end` as zeros.
 template <int D, int ROWS, int NW>
@@ -120,7 +129,7 @@ __device__ __forceinline__ void at_stage(const uint16_t* src, long ld, int r0, i
     const int g = wave + NW * i;
     if (N % NW != 0 && g >= N) break;
     const int row = RPI * g + rr;
-    const uint16_t* gp = src + (long)(r0 + row) * ld + ((p ^ at_swz(row)) << 3);
+    const uint16_t* gp = src + (long)(r0 + row) * ld + ((p ^ at_swz<D>(row)) << 3);
     if (r0 + row >= end) gp = reinterpret_cast<const uint16_t*>(&at_zero);
     __builtin_amdgcn_global_load_lds((const void*)gp, (at_lds_t)(dst + g * RPI * D), 16, 0, 0);
   }
@@ -129,7 +138,7 @@ __device__ __forceinline__ void at_stage(const uint16_t* src, long ld, int r0, i
 // Row operand: row `row` of the tile, k-values 16 s + 8 h + 0..7.
 template <int D>
 __device__ __forceinline__ u16x8 at_row(const uint16_t* tile, int row, int s, int h) {
-  return *reinterpret_cast<const u16x8*>(tile + row * D + (((2 * s + h) ^ at_swz(row)) << 3));
+  return *reinterpret_cast<const u16x8*>(tile + row * D + (((2 * s + h) ^ at_swz<D>(row)) << 3));
 }
 
 // Column operand: column 32 dt + (lane & 31), k-values = rows r0 + 8 (j >> 2) + 4 h + (j & 3).
@@ -138,9 +147,9 @@ __device__ __forceinline__ u16x8 at_col(const uint16_t* tile, int r0, int dt, in
   const int i = lane & 15, ch = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
   const int row = r0 + 4 * (lane >> 5) + (i >> 2);
   const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (at_tr_t)(tile + row * D + ((ch ^ at_swz(row)) << 3) + ((i & 1) << 2)));
+      (at_tr_t)(tile + row * D + ((ch ^ at_swz<D>(row)) << 3) + ((i & 1) << 2)));
   const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (at_tr_t)(tile + (row + 8) * D + ((ch ^ at_swz(row + 8)) << 3) + ((i & 1) << 2)));
+      (at_tr_t)(tile + (row + 8) * D + ((ch ^ at_swz<D>(row + 8)) << 3) + ((i & 1) << 2)));
   const s16x4 both[2] = {lo, hi};
   u16x8 r;
   __builtin_memcpy(&r, both, 16);

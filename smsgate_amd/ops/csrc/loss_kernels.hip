@@ -64,7 +64,8 @@ struct LossArgs {
   long ignore;
   int N, V, H, Mp, Hp, is64, mode;  // mode 0 mean, 1 sum, 2 none
   int v0, vn, ldd;                  // piece: first row, rows (of them < V - v0 real), stride of d
-  int splits, first;
+  int splits, want, most, first;    // dh: shares of Mp rows in the workspace; blocks wanted; splits at most
+  int bl, nr;                       // dh: rows of a tile, tiles over H
 };
 
 template <bool BF>
@@ -102,6 +103,16 @@ __device__ __forceinline__ uint2 lk_pack4(float a, float b, float c, float d) {
                     (uint32_t)lk_round<BF>(c) | ((uint32_t)lk_round<BF>(d) << 16));
 }
 
+// Eight values 8 e + 4 h + 0..3 (e: a pair of groups) of a row held by lanes l and l ^ 32:
+// the halves trade, so that each lane writes 16 bytes (half 0 group e, half 1 group e + 1).
+template <bool BF>
+__device__ __forceinline__ uint4 lk_trade(float4 x, float4 y) {
+  const uint2 p = lk_pack4<BF>(x.x, x.y, x.z, x.w), q = lk_pack4<BF>(y.x, y.y, y.z, y.w);
+  const auto a = __builtin_amdgcn_permlane32_swap(p.x, q.x, false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(p.y, q.y, false, false);
+  return make_uint4(a[0], b[0], a[1], b[1]);
+}
+
 __device__ __forceinline__ float lk_max_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -113,7 +124,25 @@ __device__ __forceinline__ float lk_sum_halves(float x) {
 
 __device__ __forceinline__ float lk_exp(float x) { return __builtin_amdgcn_exp2f(x * LK_LOG2E); }
 
-__device__ __forceinline__ int lk_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+__device__ __forceinline__ float4 lk_four(const f32x16& x, int e, float f) {
+  return make_float4(x[4 * e] * f, x[4 * e + 1] * f, x[4 * e + 2] * f, x[4 * e + 3] * f);
+}
+
+// What is XORed into the 16-byte chunk index of tile row `row`, for rows of CPR chunks.  LDS
+// serves 256 bytes a cycle over 64 banks: 16 lanes of a row read (16 rows, one chunk) or 32
+// of a transposing read (4 rows, 4 chunks), each conflict-free if those chunks differ modulo
+// 256 bytes.
+template <int CPR>
+__device__ __forceinline__ int lk_swz(int row) {
+  if constexpr (CPR == 8)  // 128-byte rows: row & 1 is half of the banks already
+    return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) | ((row >> 3) & 1) << 1;
+  else if constexpr (CPR % 16 == 0)
+    return (row & 3) << 2;
+  else {
+    static_assert(CPR % 16 == 8, "rows of whole 128 bytes");
+    return ((row >> 1) & 1) << 2;
+  }
+}
 
 // ---- rows with a label -----------------------------------------------------------------
 // One block: places of the labelled rows, in order.  A label outside [0, V) becomes -2 (its
@@ -180,7 +209,7 @@ __global__ void __launch_bounds__(256) loss_gather_kernel(LossArgs a) {
 // ---- products --------------------------------------------------------------------------
 // Row operand: row `row` of a [rows][64] tile, k-values 16 s + 8 h + 0..7.
 __device__ __forceinline__ u16x8 lk_row(const uint16_t* tile, int row, int s, int h) {
-  return *reinterpret_cast<const u16x8*>(tile + row * LK_K + (((2 * s + h) ^ lk_swz(row)) << 3));
+  return *reinterpret_cast<const u16x8*>(tile + row * LK_K + (((2 * s + h) ^ lk_swz<LK_K / 8>(row)) << 3));
 }
 
 // Column operand: column c0 + (lane & 31) of a [64][COLS] tile, the same k-values (its rows).
@@ -189,9 +218,9 @@ __device__ __forceinline__ u16x8 lk_col(const uint16_t* tile, int c0, int s, int
   const int i = lane & 15, ch = (c0 >> 3) + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
   const int row = 16 * s + 8 * (lane >> 5) + (i >> 2);
   const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lk_tr_t)(tile + row * COLS + ((ch ^ lk_swz(row)) << 3) + ((i & 1) << 2)));
+      (lk_tr_t)(tile + row * COLS + ((ch ^ lk_swz<COLS / 8>(row)) << 3) + ((i & 1) << 2)));
   const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lk_tr_t)(tile + (row + 4) * COLS + ((ch ^ lk_swz(row + 4)) << 3) + ((i & 1) << 2)));
+      (lk_tr_t)(tile + (row + 4) * COLS + ((ch ^ lk_swz<COLS / 8>(row + 4)) << 3) + ((i & 1) << 2)));
   const s16x4 both[2] = {lo, hi};
   u16x8 r;
   __builtin_memcpy(&r, both, 16);
@@ -212,7 +241,7 @@ struct LkStage {
     ld = ld_;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int q = (wave + NW * i) * 64 + lane, row = q / CPR, c = (q % CPR) ^ lk_swz(row);
+      const int q = (wave + NW * i) * 64 + lane, row = q / CPR, c = (q % CPR) ^ lk_swz<CPR>(row);
       const int side = COL ? r0 + 8 * c : r0 + row;
       k[i] = COL ? row : 8 * c;
       in[i] = side < rend;
@@ -229,6 +258,15 @@ struct LkStage {
   }
 };
 
+// Splits of the piece's columns that dh's share is taken in, for `tiles` tiles over `rows`
+// rows: enough blocks for the card, as many as the workspace holds.  The same for every
+// piece, so that later pieces add to the shares of the first.
+__device__ __forceinline__ int lk_splits(int rows, int tiles, const LossArgs& a) {
+  if (rows == 0) return 1;
+  const int fit = (int)((long)a.splits * a.Mp / rows), want = (a.want + tiles - 1) / tiles;
+  return max(1, min(min(fit, want), a.most));
+}
+
 // MODE 0 / 1: lane side = hidden rows, register side = vocabulary rows, k = H.
 // MODE 2: lane = the piece's vocabulary rows, register = H, k = hidden rows.
 // MODE 3: lane = hidden rows, register = H, k = a split of the piece.
@@ -242,14 +280,17 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int wl = wave / WR, wr = wave % WR;
   const int cnt = a.cnt[0];
-  const int nl = (MODE == 2 ? a.vn : a.Mp) / BL;
+  const int nl = MODE == 2 ? a.vn / BL : (cnt + BL - 1) / BL;
   const int nr = MODE >= 2 ? (a.H + BR - 1) / BR : a.vn / BR;
+  const int splits = MODE == 3 ? lk_splits(nl * BL, nl * nr, a) : 1;
   // blocks go round the 8 XCDs: each gets a run of tiles, walked in bands of 8 lane-side
-  // tiles, so that what an XCD has in flight shares its L2
+  // tiles, so that what an XCD has in flight shares its L2.  Runs of the labelled rows'
+  // tiles only (the grid holds all rows'): else a few XCDs would have all the work
   int t, z = 0;
   {
-    const int T = nl * nr * (MODE == 3 ? a.splits : 1), x = blockIdx.x & 7, q = T >> 3, r = T & 7;
-    t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
+    const int T = nl * nr * splits, x = blockIdx.x & 7, q = T >> 3, r = T & 7, i = blockIdx.x >> 3;
+    if (i >= q + (x < r)) return;
+    t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
   }
   if constexpr (MODE == 3) {
     z = t / (nl * nr);
@@ -257,11 +298,10 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   }
   const int band = t / (8 * nr), bl = t - band * 8 * nr, bw = min(8, nl - 8 * band);
   const int l0 = (8 * band + bl % bw) * BL, r0 = (bl / bw) * BR;
-  if (MODE != 2 && l0 >= cnt) return;
   int kb = 0, ke = a.Hp;
   if constexpr (MODE == 2) ke = (cnt + LK_K - 1) / LK_K * LK_K;
   if constexpr (MODE == 3) {
-    const int per = (a.vn / LK_K + a.splits - 1) / a.splits * LK_K;
+    const int per = (a.vn / LK_K + splits - 1) / splits * LK_K;
     kb = min(a.vn, z * per);
     ke = min(a.vn, kb + per);
   }
@@ -359,7 +399,7 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
       const float w = (a.w != nullptr && n < cnt ? a.w[n] : 1.f) * (BF ? 1.f : LK_FP16);
       const int y = (n < cnt ? a.lab[n] : -1) - a.v0 - rn;  // its place in this lane's registers
       const bool here = y >= 0 && y < TR;
-      uint16_t* row = a.d + (size_t)n * a.ldd + rn;
+      uint16_t* row = a.d + (size_t)n * a.ldd + (rn - 4 * h);
 #pragma unroll
       for (int i = 0; i < FR; ++i) {
 #pragma unroll
@@ -375,10 +415,9 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
             if (rn + 32 * i + 8 * (r >> 2) + (r & 3) >= vend) acc[i][j][r] = 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<uint2*>(row + 32 * i + 8 * e) =
-              lk_pack4<BF>(acc[i][j][4 * e] * w, acc[i][j][4 * e + 1] * w, acc[i][j][4 * e + 2] * w,
-                           acc[i][j][4 * e + 3] * w);
+        for (int e = 0; e < 4; e += 2)
+          *reinterpret_cast<uint4*>(row + 32 * i + 8 * (e + h)) =
+              lk_trade<BF>(lk_four(acc[i][j], e, w), lk_four(acc[i][j], e + 1, w));
       }
     }
   } else {
@@ -388,19 +427,19 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
 #pragma unroll
     for (int j = 0; j < FL; ++j) {
       const int n = ln + 32 * j;
-      if (MODE == 2 && a.v0 + n >= a.V) continue;
 #pragma unroll
       for (int i = 0; i < FR; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int c = rn + 32 * i + 8 * e;
-          if (c >= a.H) continue;
           if constexpr (MODE == 2) {
-            *reinterpret_cast<uint2*>(a.dtable + (size_t)(a.v0 + n) * a.H + c) =
-                lk_pack4<BF>(acc[i][j][4 * e] * f, acc[i][j][4 * e + 1] * f, acc[i][j][4 * e + 2] * f,
-                             acc[i][j][4 * e + 3] * f);
-          } else {
-            float4* p = reinterpret_cast<float4*>(a.share + ((size_t)z * a.Mp + n) * a.Hp + c);
+            if (e & 1) continue;
+            const uint4 x = lk_trade<BF>(lk_four(acc[i][j], e, f), lk_four(acc[i][j], e + 1, f));
+            const int c8 = c + 4 * h;  // group e, in half 1 group e + 1
+            if (a.v0 + n < a.V && c8 < a.H)
+              *reinterpret_cast<uint4*>(a.dtable + (size_t)(a.v0 + n) * a.H + c8) = x;
+          } else if (c < a.H) {
+            float4* p = reinterpret_cast<float4*>(a.share + ((size_t)z * nl * BL + n) * a.Hp + c);
             float4 x = make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
             if (!a.first) {
               const float4 y = *p;
@@ -522,8 +561,10 @@ __global__ void __launch_bounds__(256) loss_dh_kernel(LossArgs a) {
   const int row = (int)(i / nch), c = (int)(i - (long)row * nch) * 4, m = a.pos[row];
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (m >= 0) {
-    for (int z = 0; z < a.splits; ++z) {
-      const float4 x = *reinterpret_cast<const float4*>(a.share + ((size_t)z * a.Mp + m) * a.Hp + c);
+    const int rows = (a.cnt[0] + a.bl - 1) / a.bl * a.bl;
+    const int splits = lk_splits(rows, rows / a.bl * a.nr, a);
+    for (int z = 0; z < splits; ++z) {
+      const float4 x = *reinterpret_cast<const float4*>(a.share + ((size_t)z * rows + m) * a.Hp + c);
       s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
     }
     const float f = (a.mode == 2 ? a.gmax[0] : a.mode == 1 ? a.g[0] : a.g[0] / (float)a.cnt[0]) *
@@ -537,9 +578,11 @@ __global__ void __launch_bounds__(256) loss_dh_kernel(LossArgs a) {
 // Big tiles (256 x 256, 8 waves) read 3 KB of LDS per 4 products; a few hundred rows leave
 // most of the card without one, so there 64 x 64 tiles of 4 waves run instead.
 struct LossPlan {
-  int Mp, Hp, small, vtiles, piece, splits;
+  int Mp, Hp, small, vtiles, piece, splits, want, most;
 };
 
+constexpr int LK_SKEW = 64;  // on d's row stride: rows a power of two apart meet on one memory channel
+constexpr int LK_BL = 256;  // lane side of the gradients' big tiles
 constexpr long LK_PIECE = 1L << 27;  // elements of d (256 MB: what the last-level cache holds)
 
 LossPlan lk_plan(int N, int V, int H) {
@@ -553,13 +596,21 @@ LossPlan lk_plan(int N, int V, int H) {
   if (piece < 4 * LK_PAD) piece = 4 * LK_PAD;
   p.piece = (int)(piece < vp ? piece : vp);
   // dh: blocks over the card, each with at least 4 steps of k
-  const int bl = p.small ? 64 : 256, br = p.small ? 64 : 192;
+  const int bl = p.small ? 64 : LK_BL, br = p.small ? 64 : 192;
   const int tiles = p.Mp / bl * ((H + br - 1) / br);
-  int s = (512 + tiles - 1) / tiles;
-  const int most = p.piece / (4 * LK_K);
-  p.splits = s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s;
-  if (p.splits > 64) p.splits = 64;
+  p.want = 512;
+  p.most = p.piece / (4 * LK_K) < 64 ? p.piece / (4 * LK_K) : 64;
+  const int s = (p.want + tiles - 1) / tiles;
+  p.splits = s < p.most ? s : p.most;
   return p;
+}
+
+// dh: as many blocks as any count of rows may want (lk_splits: tiles x splits is at most
+// tiles + want, and at most the workspace's shares)
+unsigned lk_grid(int mode, int nl, int nr, const LossArgs& a) {
+  if (mode != 3) return (unsigned)(nl * nr);
+  const long all = (long)nl * nr * a.splits, some = (long)nl * nr + a.want;
+  return (unsigned)(((all < some ? all : some) + 7) / 8 * 8);
 }
 
 template <bool BF, int MODE>
@@ -567,13 +618,13 @@ void lk_gemm(const LossArgs& a, const LossPlan& p, hipStream_t st) {
   if (p.small) {
     const int nl = (MODE == 2 ? a.vn : a.Mp) / 64, nr = MODE >= 2 ? (a.H + 63) / 64 : a.vn / 64;
     loss_gemm_kernel<BF, MODE, 64, 64, 2, 2>
-        <<<dim3(nl * nr * (MODE == 3 ? a.splits : 1)), dim3(256), 0, st>>>(a);
+        <<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
   } else if constexpr (MODE <= 1) {
     loss_gemm_kernel<BF, MODE, 256, 256, 2, 4><<<dim3(a.Mp / 256 * (a.vn / 256)), dim3(512), 0, st>>>(a);
   } else {
-    const int nl = (MODE == 2 ? a.vn : a.Mp) / 256, nr = (a.H + 191) / 192;
-    loss_gemm_kernel<BF, MODE, 256, 192, 4, 2>
-        <<<dim3(nl * nr * (MODE == 3 ? a.splits : 1)), dim3(512), 0, st>>>(a);
+    const int nl = (MODE == 2 ? a.vn : a.Mp) / LK_BL, nr = (a.H + 191) / 192;
+    loss_gemm_kernel<BF, MODE, LK_BL, 192, LK_BL / 64, 2>
+        <<<dim3(lk_grid(MODE, nl, nr, a)), dim3(LK_BL * 2), 0, st>>>(a);
   }
 }
 
@@ -591,8 +642,9 @@ void lk_forward(LossArgs a, const LossPlan& p, hipStream_t st) {
 template <bool BF>
 void lk_backward(LossArgs a, const LossPlan& p, hipStream_t st) {
   if (a.mode == 2) loss_weights_kernel<<<dim3(1), dim3(1024), 0, st>>>(a, const_cast<float*>(a.gmax));
-  a.ldd = p.piece;
-  a.splits = p.splits;
+  a.ldd = p.piece + LK_SKEW;
+  a.splits = p.splits, a.want = p.want, a.most = p.most;
+  a.bl = p.small ? 64 : LK_BL, a.nr = p.small ? (a.H + 63) / 64 : (a.H + 191) / 192;
   const int vp = p.vtiles * (p.small ? 64 : 256);
   for (int v0 = 0; v0 < vp; v0 += p.piece) {
     a.v0 = v0;
@@ -637,7 +689,7 @@ int sg_loss_plan(int N, int V, int H, void* out) {
   o[1] = p.Hp;
   o[2] = (64 + 4 * p.Mp + N + 63) / 64;
   o[3] = (int)((2L * p.vtiles * p.Mp + 63) / 64);
-  o[4] = (int)((64 + p.Mp + (long)p.Mp * p.piece / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
+  o[4] = (int)((64 + p.Mp + (long)p.Mp * (p.piece + LK_SKEW) / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
   return 0;
 }
 
@@ -669,7 +721,7 @@ int sg_loss_bwd(const void* hc, const void* table, void* state, const void* g, v
   a.gmax = w;
   a.w = mode == 2 ? w + 64 : nullptr;
   a.d = (uint16_t*)(w + 64 + p.Mp);
-  a.share = w + 64 + p.Mp + (size_t)p.Mp * p.piece / 2;
+  a.share = w + 64 + p.Mp + (size_t)p.Mp * (p.piece + LK_SKEW) / 2;
   fp16 ? lk_backward<false>(a, p, st) : lk_backward<true>(a, p, st);
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
