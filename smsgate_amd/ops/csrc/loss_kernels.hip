@@ -50,8 +50,6 @@ constexpr int LK_K = 64;         // k-values of a staged tile
 constexpr int LK_PAD = 256;      // rows and pieces are padded to whole tiles
 constexpr float LK_FP16 = 1024.f;  // factor on d in fp16
 
-__device__ const uint4 lk_zero = {0, 0, 0, 0};
-
 struct LossArgs {
   const uint16_t *h, *table;
   const void* labels;
@@ -227,33 +225,50 @@ __device__ __forceinline__ u16x8 lk_col(const uint16_t* tile, int c0, int s, int
   return r;
 }
 
-// Copies a [rows R0 ..][64 k] or (COL) [64 k][columns C0 ..] tile by DMA; what lies outside
-// (`rend` rows, `kend` k-values; COL: `rend` columns) is read as zeros.  SIDE rows or columns.
+// Copies a [rows r0 ..][64 k] or (COL) [64 k][columns r0 ..] tile of SIDE rows or columns by
+// DMA.  Nothing outside the matrix is read: rows or columns from `rend` on repeat the last
+// one (their results are masked or not stored), k-values from `kend` on another of the same
+// row or column (the other operand holds zeros there; every step has k0 < kend).  Offsets of 32 bits from a base that
+// is the same for the wave: a step costs one scalar addition and the copies themselves.
 template <int SIDE, int NW, bool COL>
 struct LkStage {
   static constexpr int CPR = COL ? SIDE / 8 : LK_K / 8;  // chunks a tile row
   static constexpr int N = SIDE * LK_K / 512 / NW;       // DMA instructions a wave
   static_assert(SIDE * LK_K % (512 * NW) == 0, "whole instructions a wave");
-  const uint16_t* base[N];
-  int k[N], ld;
-  bool in[N];
+  const char* base;
+  uint32_t off[N];
+  int ld;  // bytes
+  __device__ __forceinline__ static int chunk(int i, int wave, int lane, int& row) {
+    const int q = (wave + NW * i) * 64 + lane;
+    row = q / CPR;
+    return (q % CPR) ^ lk_swz<CPR>(row);
+  }
   __device__ __forceinline__ void init(const uint16_t* src, int ld_, int r0, int rend, int wave, int lane) {
-    ld = ld_;
+    ld = 2 * ld_;
+    const int rb = COL ? min(r0, rend - 8) : min(r0, rend - 1);
+    base = reinterpret_cast<const char*>(src) + (COL ? 2 * (long)rb : (long)rb * ld);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int q = (wave + NW * i) * 64 + lane, row = q / CPR, c = (q % CPR) ^ lk_swz<CPR>(row);
-      const int side = COL ? r0 + 8 * c : r0 + row;
-      k[i] = COL ? row : 8 * c;
-      in[i] = side < rend;
-      base[i] = src + (COL ? (size_t)row * ld + side : (size_t)side * ld + k[i]);
+      int row;
+      const int c = chunk(i, wave, lane, row);
+      off[i] = COL ? (uint32_t)(row * ld + 2 * (min(r0 + 8 * c, rend - 8) - rb))
+                   : (uint32_t)((min(r0 + row, rend - 1) - rb) * ld + 16 * c);
     }
   }
-  __device__ __forceinline__ void issue(uint16_t* dst, int k0, int kend, int wave) const {
+  __device__ __forceinline__ void issue(uint16_t* dst, int k0, int kend, int wave, int lane) const {
+    const char* p = base + (COL ? (long)k0 * ld : 2 * (long)k0);
+    if (k0 + LK_K <= kend) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint16_t* p = base[i] + (COL ? (size_t)k0 * ld : (size_t)k0);
-      if (!in[i] || k0 + k[i] >= kend) p = reinterpret_cast<const uint16_t*>(&lk_zero);
-      __builtin_amdgcn_global_load_lds((const void*)p, (lk_lds_t)(dst + (wave + NW * i) * 512), 16, 0, 0);
+      for (int i = 0; i < N; ++i)
+        __builtin_amdgcn_global_load_lds((const void*)(p + off[i]), (lk_lds_t)(dst + (wave + NW * i) * 512), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        int row;
+        const int c = chunk(i, wave, lane, row), over = (COL ? row : 8 * c) - (kend - 1 - k0);
+        const uint32_t o = off[i] - (over <= 0 ? 0u : (uint32_t)(COL ? over * ld : 16 * c));
+        __builtin_amdgcn_global_load_lds((const void*)(p + o), (lk_lds_t)(dst + (wave + NW * i) * 512), 16, 0, 0);
+      }
     }
   }
 };
@@ -302,8 +317,10 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   if constexpr (MODE == 2) ke = (cnt + LK_K - 1) / LK_K * LK_K;
   if constexpr (MODE == 3) {
     const int per = (a.vn / LK_K + splits - 1) / splits * LK_K;
-    kb = min(a.vn, z * per);
-    ke = min(a.vn, kb + per);
+    // steps wholly behind the vocabulary are left out: d is zero there, and E has no such rows
+    const int end = (min(a.vn, a.V - a.v0) + LK_K - 1) / LK_K * LK_K;
+    kb = min(end, z * per);
+    ke = min(end, kb + per);
   }
   LkStage<BL, NW, LCOL> sl;
   LkStage<BR, NW, RCOL> sr;
@@ -320,8 +337,8 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   const int kl = MODE == 3 ? a.vn : MODE == 2 ? a.Mp : a.Hp;                  // k-values that exist
   const int kr = MODE == 3 ? min(a.vn, a.V - a.v0) : MODE == 2 ? a.Mp : a.H;
   auto stage = [&](int k0, int buf) {
-    sl.issue(sm + buf * STAGE, k0, kl, wave);
-    sr.issue(sm + buf * STAGE + BL * LK_K, k0, kr, wave);
+    sl.issue(sm + buf * STAGE, k0, kl, wave, lane);
+    sr.issue(sm + buf * STAGE + BL * LK_K, k0, kr, wave, lane);
   };
   f32x16 acc[FR][FL];
 #pragma unroll
@@ -337,19 +354,26 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
     asm volatile("" ::: "memory");
     if (k0 + LK_K < ke) stage(k0 + LK_K, buf ^ 1);
     const uint16_t *ls = sm + buf * STAGE, *rs = ls + BL * LK_K;
-#pragma unroll
-    for (int s = 0; s < LK_K / 16; ++s) {
-      u16x8 lf[FL], rf[FR];
+    // the operands of the next 16 k-values are read while these are multiplied
+    u16x8 lf[2][FL], rf[2][FR];
+    auto read = [&](int s) {
 #pragma unroll
       for (int j = 0; j < FL; ++j)
-        lf[j] = LCOL ? lk_col<BL>(ls, wl * TL + 32 * j, s, lane) : lk_row(ls, wl * TL + 32 * j + (lane & 31), s, h);
+        lf[s & 1][j] =
+            LCOL ? lk_col<BL>(ls, wl * TL + 32 * j, s, lane) : lk_row(ls, wl * TL + 32 * j + (lane & 31), s, h);
 #pragma unroll
       for (int i = 0; i < FR; ++i)
-        rf[i] = RCOL ? lk_col<BR>(rs, wr * TR + 32 * i, s, lane) : lk_row(rs, wr * TR + 32 * i + (lane & 31), s, h);
+        rf[s & 1][i] =
+            RCOL ? lk_col<BR>(rs, wr * TR + 32 * i, s, lane) : lk_row(rs, wr * TR + 32 * i + (lane & 31), s, h);
+    };
+    read(0);
+#pragma unroll
+    for (int s = 0; s < LK_K / 16; ++s) {
+      if (s + 1 < LK_K / 16) read(s + 1);
 #pragma unroll
       for (int i = 0; i < FR; ++i)
 #pragma unroll
-        for (int j = 0; j < FL; ++j) acc[i][j] = lk_mma<BF>(rf[i], lf[j], acc[i][j]);
+        for (int j = 0; j < FL; ++j) acc[i][j] = lk_mma<BF>(rf[s & 1][i], lf[s & 1][j], acc[i][j]);
     }
   }
   // register r of acc[i][j]: register-side index r0 + wr TR + 32 i + 8 (r >> 2) + 4 h + (r & 3)
