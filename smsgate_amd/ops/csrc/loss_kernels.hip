@@ -46,7 +46,7 @@ typedef __attribute__((address_space(3))) void* lk_lds_t;
 typedef __attribute__((address_space(3))) s16x4* lk_tr_t;
 
 constexpr float LK_LOG2E = 1.4426950408889634f;
-constexpr int LK_K = 64;         // k-values of a staged tile
+constexpr int LK_K = 64;         // hc's columns and dh's splits are whole multiples
 constexpr int LK_PAD = 256;      // rows and pieces are padded to whole tiles
 constexpr float LK_FP16 = 1024.f;  // factor on d in fp16
 
@@ -61,7 +61,7 @@ struct LossArgs {
   const float *g, *gmax;            // incoming gradient; none: its largest magnitude
   long ignore;
   int N, V, H, Mp, Hp, is64, mode;  // mode 0 mean, 1 sum, 2 none
-  int v0, vn, ldd;                  // piece: first row, rows (of them < V - v0 real), stride of d
+  int v0, vn;                       // piece: first row, rows (of them < V - v0 real)
   int splits, want, most, first;    // dh: shares of Mp rows in the workspace; blocks wanted; splits at most
   int bl, nr;                       // dh: rows of a tile, tiles over H
 };
@@ -132,7 +132,9 @@ __device__ __forceinline__ float4 lk_four(const f32x16& x, int e, float f) {
 // 256 bytes.
 template <int CPR>
 __device__ __forceinline__ int lk_swz(int row) {
-  if constexpr (CPR == 8)  // 128-byte rows: row & 1 is half of the banks already
+  if constexpr (CPR == 4)  // 64-byte rows: row & 3 is a quarter of the banks already
+    return (row >> 2) & 3;
+  else if constexpr (CPR == 8)  // 128-byte rows: row & 1 is half of the banks already
     return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) | ((row >> 3) & 1) << 1;
   else if constexpr (CPR % 16 == 0)
     return (row & 3) << 2;
@@ -205,12 +207,13 @@ __global__ void __launch_bounds__(256) loss_gather_kernel(LossArgs a) {
 }
 
 // ---- products --------------------------------------------------------------------------
-// Row operand: row `row` of a [rows][64] tile, k-values 16 s + 8 h + 0..7.
+// Row operand: row `row` of a [rows][BK] tile, k-values 16 s + 8 h + 0..7.
+template <int BK>
 __device__ __forceinline__ u16x8 lk_row(const uint16_t* tile, int row, int s, int h) {
-  return *reinterpret_cast<const u16x8*>(tile + row * LK_K + (((2 * s + h) ^ lk_swz<LK_K / 8>(row)) << 3));
+  return *reinterpret_cast<const u16x8*>(tile + row * BK + (((2 * s + h) ^ lk_swz<BK / 8>(row)) << 3));
 }
 
-// Column operand: column c0 + (lane & 31) of a [64][COLS] tile, the same k-values (its rows).
+// Column operand: column c0 + (lane & 31) of a [BK][COLS] tile, the same k-values (its rows).
 template <int COLS>
 __device__ __forceinline__ u16x8 lk_col(const uint16_t* tile, int c0, int s, int lane) {
   const int i = lane & 15, ch = (c0 >> 3) + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
@@ -225,16 +228,17 @@ __device__ __forceinline__ u16x8 lk_col(const uint16_t* tile, int c0, int s, int
   return r;
 }
 
-// Copies a [rows r0 ..][64 k] or (COL) [64 k][columns r0 ..] tile of SIDE rows or columns by
+// Copies a [rows r0 ..][BK k] or (COL) [BK k][columns r0 ..] tile of SIDE rows or columns by
 // DMA.  Nothing outside the matrix is read: rows or columns from `rend` on repeat the last
-// one (their results are masked or not stored), k-values from `kend` on another of the same
-// row or column (the other operand holds zeros there; every step has k0 < kend).  Offsets of 32 bits from a base that
-// is the same for the wave: a step costs one scalar addition and the copies themselves.
-template <int SIDE, int NW, bool COL>
+// one (their results are masked or not stored), k-values from the `rem`-th on another of the
+// same row or column (the other operand holds zeros there; rem >= 1).  Offsets of 32 bits
+// from a base that is the same for the wave: a step costs one scalar addition and the copies
+// themselves.
+template <int SIDE, int NW, bool COL, int BK>
 struct LkStage {
-  static constexpr int CPR = COL ? SIDE / 8 : LK_K / 8;  // chunks a tile row
-  static constexpr int N = SIDE * LK_K / 512 / NW;       // DMA instructions a wave
-  static_assert(SIDE * LK_K % (512 * NW) == 0, "whole instructions a wave");
+  static constexpr int CPR = COL ? SIDE / 8 : BK / 8;  // chunks a tile row
+  static constexpr int N = SIDE * BK / 512 / NW;       // DMA instructions a wave
+  static_assert(SIDE * BK % (512 * NW) == 0, "whole instructions a wave");
   const char* base;
   uint32_t off[N];
   int ld;  // bytes
@@ -255,9 +259,10 @@ struct LkStage {
                    : (uint32_t)((min(r0 + row, rend - 1) - rb) * ld + 16 * c);
     }
   }
-  __device__ __forceinline__ void issue(uint16_t* dst, int k0, int kend, int wave, int lane) const {
-    const char* p = base + (COL ? (long)k0 * ld : 2 * (long)k0);
-    if (k0 + LK_K <= kend) {
+  // at: byte offset of the step's first k-value
+  __device__ __forceinline__ void issue(uint16_t* dst, long at, int rem, int wave, int lane) const {
+    const char* p = base + at;
+    if (rem >= BK) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
         __builtin_amdgcn_global_load_lds((const void*)(p + off[i]), (lk_lds_t)(dst + (wave + NW * i) * 512), 16, 0, 0);
@@ -265,7 +270,7 @@ struct LkStage {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         int row;
-        const int c = chunk(i, wave, lane, row), over = (COL ? row : 8 * c) - (kend - 1 - k0);
+        const int c = chunk(i, wave, lane, row), over = (COL ? row : 8 * c) - (rem - 1);
         const uint32_t o = off[i] - (over <= 0 ? 0u : (uint32_t)(COL ? over * ld : 16 * c));
         __builtin_amdgcn_global_load_lds((const void*)(p + o), (lk_lds_t)(dst + (wave + NW * i) * 512), 16, 0, 0);
       }
@@ -282,16 +287,23 @@ __device__ __forceinline__ int lk_splits(int rows, int tiles, const LossArgs& a)
   return max(1, min(min(fit, want), a.most));
 }
 
+// d lies in panels of LK_PANEL columns, [panel][Mp][LK_PANEL]: a tile of it is one run of
+// memory whichever way it is read (rows of the whole piece, 32 KB apart, cost 2 us a step).
+constexpr int LK_PANEL = 256;
+
 // MODE 0 / 1: lane side = hidden rows, register side = vocabulary rows, k = H.
 // MODE 2: lane = the piece's vocabulary rows, register = H, k = hidden rows.
 // MODE 3: lane = hidden rows, register = H, k = a split of the piece.
-template <bool BF, int MODE, int BL, int BR, int WL, int WR>
+// BK k-values a step, ST buffers: the copies of the next ST - 1 steps are in flight.
+template <bool BF, int MODE, int BL, int BR, int WL, int WR, int BK, int ST>
 __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   constexpr int NW = WL * WR, TL = BL / WL, TR = BR / WR, FL = TL / 32, FR = TR / 32;
   constexpr bool LCOL = MODE == 2, RCOL = MODE >= 2;
-  constexpr int STAGE = (BL + BR) * LK_K;
-  static_assert(2 * STAGE * 2 <= 160 * 1024 && BL % (32 * WL) == 0 && BR % (32 * WR) == 0, "tile");
-  __shared__ __attribute__((aligned(16))) uint16_t sm[2 * STAGE];
+  constexpr int STAGE = (BL + BR) * BK;
+  static_assert(ST * STAGE * 2 <= 160 * 1024 && BL % (32 * WL) == 0 && BR % (32 * WR) == 0, "tile");
+  static_assert(LK_PANEL % BL == 0 || MODE != 2, "d's columns of a tile lie in one panel");
+  static_assert(LK_PANEL % BR == 0 || MODE != 1, "d's columns of a tile lie in one panel");
+  __shared__ __attribute__((aligned(16))) uint16_t sm[ST * STAGE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int wl = wave / WR, wr = wave % WR;
   const int cnt = a.cnt[0];
@@ -313,63 +325,78 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   }
   const int band = t / (8 * nr), bl = t - band * 8 * nr, bw = min(8, nl - 8 * band);
   const int l0 = (8 * band + bl % bw) * BL, r0 = (bl / bw) * BR;
-  int kb = 0, ke = a.Hp;
-  if constexpr (MODE == 2) ke = (cnt + LK_K - 1) / LK_K * LK_K;
+  int kb = 0, ke = (a.H + BK - 1) / BK * BK;
+  if constexpr (MODE == 2) ke = (cnt + BK - 1) / BK * BK;
   if constexpr (MODE == 3) {
     const int per = (a.vn / LK_K + splits - 1) / splits * LK_K;
     // steps wholly behind the vocabulary are left out: d is zero there, and E has no such rows
-    const int end = (min(a.vn, a.V - a.v0) + LK_K - 1) / LK_K * LK_K;
+    const int end = (min(a.vn, a.V - a.v0) + BK - 1) / BK * BK;
     kb = min(end, z * per);
     ke = min(end, kb + per);
   }
-  LkStage<BL, NW, LCOL> sl;
-  LkStage<BR, NW, RCOL> sr;
+  LkStage<BL, NW, LCOL, BK> sl;
+  LkStage<BR, NW, RCOL, BK> sr;
+  const long panel = (long)a.Mp * LK_PANEL;
   if constexpr (MODE <= 1) {
     sl.init(a.hc, a.Hp, l0, a.Mp, wave, lane);
     sr.init(a.table, a.H, a.v0 + r0, a.V, wave, lane);
   } else if constexpr (MODE == 2) {
-    sl.init(a.d, a.ldd, l0, a.vn, wave, lane);
+    sl.init(a.d + l0 / LK_PANEL * panel, LK_PANEL, l0 % LK_PANEL, LK_PANEL, wave, lane);
     sr.init(a.hc, a.Hp, r0, a.Hp, wave, lane);
   } else {
-    sl.init(a.d, a.ldd, l0, a.Mp, wave, lane);
+    sl.init(a.d, LK_PANEL, l0, a.Mp, wave, lane);
     sr.init(a.table + (size_t)a.v0 * a.H, a.H, r0, a.H, wave, lane);
   }
-  const int kl = MODE == 3 ? a.vn : MODE == 2 ? a.Mp : a.Hp;                  // k-values that exist
-  const int kr = MODE == 3 ? min(a.vn, a.V - a.v0) : MODE == 2 ? a.Mp : a.H;
   auto stage = [&](int k0, int buf) {
-    sl.issue(sm + buf * STAGE, k0, kl, wave, lane);
-    sr.issue(sm + buf * STAGE + BL * LK_K, k0, kr, wave, lane);
+    uint16_t *ls = sm + buf * STAGE, *rs = ls + BL * BK;
+    if constexpr (MODE <= 1) {
+      sl.issue(ls, 2 * k0, BK, wave, lane);
+      sr.issue(rs, 2 * k0, a.H - k0, wave, lane);
+    } else if constexpr (MODE == 2) {
+      sl.issue(ls, (long)k0 * (2 * LK_PANEL), BK, wave, lane);
+      sr.issue(rs, (long)k0 * (2 * a.Hp), BK, wave, lane);
+    } else {
+      sl.issue(ls, 2 * (k0 / LK_PANEL * panel + k0 % LK_PANEL), BK, wave, lane);
+      sr.issue(rs, (long)k0 * (2 * a.H), a.V - a.v0 - k0, wave, lane);
+    }
   };
   f32x16 acc[FR][FL];
 #pragma unroll
   for (int i = 0; i < FR; ++i)
 #pragma unroll
     for (int j = 0; j < FL; ++j) acc[i][j] = (f32x16)0.f;
-  if (kb < ke) stage(kb, 0);
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i)
+    if (kb + i * BK < ke) stage(kb + i * BK, i);
   int buf = 0;
-  for (int k0 = kb; k0 < ke; k0 += LK_K, buf ^= 1) {
-    // this wave's copies have landed and its reads of the other buffer are done; every wave's
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  for (int k0 = kb; k0 < ke; k0 += BK) {
+    // this wave's copies for this step have landed (those of the ST - 2 steps behind may be
+    // under way) and its reads of the buffer before are done; then every wave's
+    if (k0 + (ST - 2) * BK < ke)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((decltype(sl)::N + decltype(sr)::N) * (ST - 2)) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (k0 + LK_K < ke) stage(k0 + LK_K, buf ^ 1);
-    const uint16_t *ls = sm + buf * STAGE, *rs = ls + BL * LK_K;
+    if (k0 + (ST - 1) * BK < ke) stage(k0 + (ST - 1) * BK, buf == 0 ? ST - 1 : buf - 1);
+    const uint16_t *ls = sm + buf * STAGE, *rs = ls + BL * BK;
+    buf = buf + 1 == ST ? 0 : buf + 1;
     // the operands of the next 16 k-values are read while these are multiplied
     u16x8 lf[2][FL], rf[2][FR];
     auto read = [&](int s) {
 #pragma unroll
       for (int j = 0; j < FL; ++j)
         lf[s & 1][j] =
-            LCOL ? lk_col<BL>(ls, wl * TL + 32 * j, s, lane) : lk_row(ls, wl * TL + 32 * j + (lane & 31), s, h);
+            LCOL ? lk_col<BL>(ls, wl * TL + 32 * j, s, lane) : lk_row<BK>(ls, wl * TL + 32 * j + (lane & 31), s, h);
 #pragma unroll
       for (int i = 0; i < FR; ++i)
         rf[s & 1][i] =
-            RCOL ? lk_col<BR>(rs, wr * TR + 32 * i, s, lane) : lk_row(rs, wr * TR + 32 * i + (lane & 31), s, h);
+            RCOL ? lk_col<BR>(rs, wr * TR + 32 * i, s, lane) : lk_row<BK>(rs, wr * TR + 32 * i + (lane & 31), s, h);
     };
     read(0);
 #pragma unroll
-    for (int s = 0; s < LK_K / 16; ++s) {
-      if (s + 1 < LK_K / 16) read(s + 1);
+    for (int s = 0; s < BK / 16; ++s) {
+      if (s + 1 < BK / 16) read(s + 1);
 #pragma unroll
       for (int i = 0; i < FR; ++i)
 #pragma unroll
@@ -423,7 +450,7 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
       const float w = (a.w != nullptr && n < cnt ? a.w[n] : 1.f) * (BF ? 1.f : LK_FP16);
       const int y = (n < cnt ? a.lab[n] : -1) - a.v0 - rn;  // its place in this lane's registers
       const bool here = y >= 0 && y < TR;
-      uint16_t* row = a.d + (size_t)n * a.ldd + (rn - 4 * h);
+      uint16_t* row = a.d + r0 / LK_PANEL * panel + (size_t)n * LK_PANEL + (r0 % LK_PANEL + wr * TR);
 #pragma unroll
       for (int i = 0; i < FR; ++i) {
 #pragma unroll
@@ -605,8 +632,7 @@ struct LossPlan {
   int Mp, Hp, small, vtiles, piece, splits, want, most;
 };
 
-constexpr int LK_SKEW = 64;  // on d's row stride: rows a power of two apart meet on one memory channel
-constexpr int LK_BL = 256;  // lane side of the gradients' big tiles
+constexpr int LK_BL = 128;  // lane side of the gradients' big tiles
 constexpr long LK_PIECE = 1L << 27;  // elements of d (256 MB: what the last-level cache holds)
 
 LossPlan lk_plan(int N, int V, int H) {
@@ -641,14 +667,12 @@ template <bool BF, int MODE>
 void lk_gemm(const LossArgs& a, const LossPlan& p, hipStream_t st) {
   if (p.small) {
     const int nl = (MODE == 2 ? a.vn : a.Mp) / 64, nr = MODE >= 2 ? (a.H + 63) / 64 : a.vn / 64;
-    loss_gemm_kernel<BF, MODE, 64, 64, 2, 2>
-        <<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
+    loss_gemm_kernel<BF, MODE, 64, 64, 2, 2, 64, 2><<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
   } else if constexpr (MODE <= 1) {
-    loss_gemm_kernel<BF, MODE, 256, 256, 2, 4><<<dim3(a.Mp / 256 * (a.vn / 256)), dim3(512), 0, st>>>(a);
+    loss_gemm_kernel<BF, MODE, 128, 256, 1, 4, 32, 3><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
   } else {
     const int nl = (MODE == 2 ? a.vn : a.Mp) / LK_BL, nr = (a.H + 191) / 192;
-    loss_gemm_kernel<BF, MODE, LK_BL, 192, LK_BL / 64, 2>
-        <<<dim3(lk_grid(MODE, nl, nr, a)), dim3(LK_BL * 2), 0, st>>>(a);
+    loss_gemm_kernel<BF, MODE, LK_BL, 192, 2, 2, 32, 4><<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
   }
 }
 
@@ -666,7 +690,6 @@ void lk_forward(LossArgs a, const LossPlan& p, hipStream_t st) {
 template <bool BF>
 void lk_backward(LossArgs a, const LossPlan& p, hipStream_t st) {
   if (a.mode == 2) loss_weights_kernel<<<dim3(1), dim3(1024), 0, st>>>(a, const_cast<float*>(a.gmax));
-  a.ldd = p.piece + LK_SKEW;
   a.splits = p.splits, a.want = p.want, a.most = p.most;
   a.bl = p.small ? 64 : LK_BL, a.nr = p.small ? (a.H + 63) / 64 : (a.H + 191) / 192;
   const int vp = p.vtiles * (p.small ? 64 : 256);
@@ -713,7 +736,7 @@ int sg_loss_plan(int N, int V, int H, void* out) {
   o[1] = p.Hp;
   o[2] = (64 + 4 * p.Mp + N + 63) / 64;
   o[3] = (int)((2L * p.vtiles * p.Mp + 63) / 64);
-  o[4] = (int)((64 + p.Mp + (long)p.Mp * (p.piece + LK_SKEW) / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
+  o[4] = (int)((64 + p.Mp + (long)p.Mp * p.piece / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
   return 0;
 }
 
@@ -745,7 +768,7 @@ int sg_loss_bwd(const void* hc, const void* table, void* state, const void* g, v
   a.gmax = w;
   a.w = mode == 2 ? w + 64 : nullptr;
   a.d = (uint16_t*)(w + 64 + p.Mp);
-  a.share = w + 64 + p.Mp + (size_t)p.Mp * (p.piece + LK_SKEW) / 2;
+  a.share = w + 64 + p.Mp + (size_t)p.Mp * p.piece / 2;
   fp16 ? lk_backward<false>(a, p, st) : lk_backward<true>(a, p, st);
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
