@@ -11,21 +11,24 @@
 // Both directions are bound by memory: the rows read, x / dx, and dE written once whole.
 //   * up to EG_SMALL entries (one message): ONE launch; every block scans all the ids for
 //     its 16 rows of dE.  A launch costs more than the work.
-//   * else the entries are sorted by id (stable, so each id's positions stay in order):
-//     up to EG_LDS entries in one block's LDS, more with three launches a pass of 8 bits;
-//     then one wave a row of dE sums its positions (rows of no entry are zeroed there, so
-//     dE is written once).  An id of many entries (a separator, the shared prompt) would
-//     leave one wave with thousands of rows: runs of EG_CHUNK sorted entries of one id are
-//     summed beforehand, and rows of over EG_COOP terms are shared by the block's 4 waves.
+//   * else the entries are sorted by id (stable, so each id's positions stay in order), in
+//     one launch up to EG_RANGE entries, else in three launches a pass of 8 bits; then one
+//     wave a row of dE sums its positions (rows of no entry are zeroed there, so dE is
+//     written once).  An id of many entries (a separator, the shared prompt) would leave
+//     one wave with thousands of rows: runs of EG_CHUNK sorted entries of one id are summed
+//     beforehand, and rows of over EG_COOP terms are shared by the block's 4 waves.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 namespace {
 
 constexpr int EG_SMALL = 256;    // entries that the one-launch gradient takes
-constexpr int EG_LDS = 16384;    // entries that one block sorts in LDS (2 x 64 KB + counters)
-constexpr int EG_IDX_BITS = 14;  // EG_LDS positions beside an 18-bit id in one word
-constexpr int EG_CHUNK = 64;     // sorted entries of one id summed beforehand
+// Entries, and ids, that the one-launch sort takes: its blocks each read every id, so its time
+// grows by 1.4 us a thousand entries (25 us at 15616, 192 at 130999), the passes' by 0.1
+// from 30 us (40 at 130999).
+constexpr int EG_RANGE = 1 << 14;
+constexpr int EG_RANGE_V = 1 << 18;
+constexpr int EG_CHUNK = 32;     // sorted entries of one id summed beforehand
 constexpr int EG_COOP = 16;      // terms of a row that one wave sums alone
 constexpr int EG_TILE = 2048;    // entries of one block of a radix pass
 
@@ -152,80 +155,87 @@ __device__ __forceinline__ void eg_wave_step(volatile int* cnt, uint32_t digit, 
   }
 }
 
-// Sorts n2 <= EG_LDS entries in one block and writes them with each id's [start, end).
-// seg is zeroed here too: an id without entries has start = end = 0.
-__global__ void __launch_bounds__(1024) embed_sort_lds_kernel(const void* __restrict__ ids,
-                                                              const void* __restrict__ add, int is64, int n, int n2,
-                                                              int V, int passes, uint32_t* __restrict__ keys,
-                                                              int* __restrict__ ents, int2* __restrict__ seg) {
-  __shared__ uint32_t buf[2 * EG_LDS];
-  __shared__ int cnt[16 * 256];  // [wave][digit]
-  __shared__ int base[256];
+// Sorts up to EG_RANGE entries in one launch: block b places the entries of the 256 ids
+// [256 b, 256 b + 256) by itself.  It reads every id twice (from L2: 8 n2 bytes a block), to
+// count its ids and the entries of lower ids, which is where its own begin, and to place
+// them; a wave owns a run of entries, so places keep their order.  Writes seg of its ids.
+__global__ void __launch_bounds__(1024) embed_range_sort_kernel(const void* __restrict__ ids,
+                                                                const void* __restrict__ add, int is64, int n, int n2,
+                                                                int V, uint32_t* __restrict__ keys,
+                                                                int* __restrict__ ents, int2* __restrict__ seg) {
+  __shared__ int cnt[16 * 256];  // [wave][id]
+  __shared__ int sum[256], low[16];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  for (int v = tid; v < V; v += 1024) seg[v] = make_int2(0, 0);
-  for (int e = tid; e < n2; e += 1024)
-    buf[e] = (eg_key(ids, add, is64, n, e, V) << EG_IDX_BITS) | (uint32_t)e;
-  const int per = ((n2 + 15) / 16 + 63) & ~63;  // entries of a wave, in order
+  const uint32_t v0 = blockIdx.x * 256;
+  const int per = ((n2 + 15) / 16 + 63) & ~63;
   const int w0 = wave * per, w1 = min(n2, w0 + per);
-  for (int p = 0; p < passes; ++p) {
-    const uint32_t* src = buf + (p & 1) * EG_LDS;
-    uint32_t* dst = buf + ((p & 1) ^ 1) * EG_LDS;
-    const int sh = EG_IDX_BITS + 8 * p;
-    volatile int* mine = cnt + wave * 256;
-    for (int i = tid; i < 16 * 256; i += 1024) cnt[i] = 0;
-    __syncthreads();
-    for (int e0 = w0; e0 < w1; e0 += 64) {
-      const bool on = e0 + lane < w1;
-      const uint32_t d = on ? (src[e0 + lane] >> sh) & 255u : 0u;
-      eg_wave_step<false>(mine, d, on, lane, [](int) {});
-    }
-    __syncthreads();
-    if (tid < 256) {  // places of a digit within it, wave by wave
-      int s = 0;
-      for (int w = 0; w < 16; ++w) {
-        const int c = cnt[w * 256 + tid];
-        cnt[w * 256 + tid] = s;
-        s += c;
-      }
-      base[tid] = s;
-    }
-    __syncthreads();
-    if (tid < 64) {  // exclusive sums over the 256 digits, 4 a lane
-      int a[4], s = 0;
+  volatile int* mine = cnt + wave * 256;
+  for (int i = tid; i < 16 * 256; i += 1024) cnt[i] = 0;
+  __syncthreads();
+  // f(entry, key, in range) for the wave's entries, 8 loads in flight
+  auto walk = [&](auto f) {
+    for (int e0 = w0; e0 < w1; e0 += 512) {
+      uint32_t k[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        a[k] = s;
-        s += base[4 * tid + k];
-      }
-      int inc = s;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += t;
+      for (int r = 0; r < 8; ++r) {
+        const int e = e0 + 64 * r + lane;
+        k[r] = e < w1 ? eg_key(ids, add, is64, n, e, V) : (uint32_t)V;
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) base[4 * tid + k] = inc - s + a[k];
+      for (int r = 0; r < 8; ++r) f(e0 + 64 * r + lane, k[r], k[r] - v0 < 256u && k[r] < (uint32_t)V);
     }
-    __syncthreads();
-    for (int i = tid; i < 16 * 256; i += 1024) cnt[i] += base[i & 255];
-    __syncthreads();
-    for (int e0 = w0; e0 < w1; e0 += 64) {
-      const bool on = e0 + lane < w1;
-      const uint32_t u = on ? src[e0 + lane] : 0u;
-      eg_wave_step<true>(mine, (u >> sh) & 255u, on, lane, [&](int at) { dst[at] = u; });
+  };
+  int below = 0;
+  walk([&](int, uint32_t k, bool on) {
+    below += k < v0;  // (an id of no row is V: in no range and below none)
+    if (__any(on)) eg_wave_step<false>(mine, (k - v0) & 255u, on, lane, [](int) {});
+  });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o, 64);
+  if (lane == 0) low[wave] = below;
+  __syncthreads();
+  if (tid < 256) {  // places of an id's entries within it, wave by wave
+    int c = 0;
+    for (int w = 0; w < 16; ++w) {
+      const int x = cnt[w * 256 + tid];
+      cnt[w * 256 + tid] = c;
+      c += x;
     }
-    __syncthreads();
+    sum[tid] = c;
   }
-  const uint32_t* res = buf + (passes & 1) * EG_LDS;
-  for (int e = tid; e < n2; e += 1024) {
-    const uint32_t u = res[e], k = u >> EG_IDX_BITS;
-    keys[e] = k;
-    ents[e] = (int)(u & (EG_LDS - 1));
-    if (k < (uint32_t)V) {  // the block's zeroes of seg were written before the first barrier
-      if (e == 0 || (res[e - 1] >> EG_IDX_BITS) != k) seg[k].x = e;
-      if (e + 1 == n2 || (res[e + 1] >> EG_IDX_BITS) != k) seg[k].y = e + 1;
+  __syncthreads();
+  if (tid < 64) {  // where each id begins: the lower ids' entries, then the range's in order
+    int base = 0;
+    for (int w = 0; w < 16; ++w) base += low[w];
+    int a[4], s = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a[k] = s;
+      s += sum[4 * tid + k];
+    }
+    int inc = s;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += t;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int x = base + inc - s + a[k], y = sum[4 * tid + k];
+      if (v0 + 4 * tid + k < (uint32_t)V) seg[v0 + 4 * tid + k] = make_int2(x, x + y);
+      sum[4 * tid + k] = x;
     }
   }
+  __syncthreads();
+  for (int i = tid; i < 16 * 256; i += 1024) cnt[i] += sum[i & 255];
+  __syncthreads();
+  walk([&](int e, uint32_t k, bool on) {
+    if (__any(on))
+      eg_wave_step<true>(mine, (k - v0) & 255u, on, lane, [&](int at) {
+        keys[at] = k;
+        ents[at] = e;
+      });
+  });
 }
 
 // Radix pass over tiles of EG_TILE entries.  The first pass reads the ids themselves.
@@ -252,42 +262,24 @@ __global__ void __launch_bounds__(256) embed_hist_kernel(const uint32_t* __restr
     for (long v = (long)blockIdx.x * 256 + tid; v < V; v += (long)gridDim.x * 256) seg[v] = make_int2(0, 0);
 }
 
-// Exclusive sums of m counters in place, one block.
-__global__ void __launch_bounds__(1024) embed_scan_kernel(int* __restrict__ hist, int m) {
-  __shared__ int part[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int carry = 0;
-  for (int i0 = 0; i0 < m; i0 += 4096) {
-    int a[4], s = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = i0 + 4 * tid + k;
-      a[k] = s;
-      s += i < m ? hist[i] : 0;
-    }
-    int inc = s;
+// Exclusive sums over the tiles of a digit in place, a wave a digit, and the digit's total
+// behind all of them (the scatter adds the lower digits' totals).
+__global__ void __launch_bounds__(256) embed_scan_kernel(int* __restrict__ hist, int tiles) {
+  const int digit = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int* row = hist + (size_t)digit * tiles;
+  int base = 0;
+  for (int t0 = 0; t0 < tiles; t0 += 64) {
+    const int x = t0 + lane < tiles ? row[t0 + lane] : 0;
+    int inc = x;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int t = __shfl_up(inc, o, 64);
       if (lane >= o) inc += t;
     }
-    if (lane == 63) part[wave] = inc;
-    __syncthreads();
-    int off = carry, all = 0;
-    for (int w = 0; w < 16; ++w) {
-      const int t = part[w];
-      if (w < wave) off += t;
-      all += t;
-    }
-    off += inc - s;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = i0 + 4 * tid + k;
-      if (i < m) hist[i] = off + a[k];
-    }
-    carry += all;
-    __syncthreads();
+    if (t0 + lane < tiles) row[t0 + lane] = base + inc - x;
+    base += __shfl(inc, 63, 64);
   }
+  if (lane == 0) hist[(size_t)256 * tiles + digit] = base;
 }
 
 __global__ void __launch_bounds__(256) embed_scatter_kernel(const uint32_t* __restrict__ keys,
@@ -297,7 +289,7 @@ __global__ void __launch_bounds__(256) embed_scatter_kernel(const uint32_t* __re
                                                             int V, int sh, const int* __restrict__ hist,
                                                             uint32_t* __restrict__ keys_out,
                                                             int* __restrict__ ents_out) {
-  __shared__ int cnt[4 * 256];
+  __shared__ int cnt[4 * 256], low[256];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int w0 = blockIdx.x * EG_TILE + wave * (EG_TILE / 4), w1 = min(n2, w0 + EG_TILE / 4);
   volatile int* mine = cnt + wave * 256;
@@ -310,9 +302,26 @@ __global__ void __launch_bounds__(256) embed_scatter_kernel(const uint32_t* __re
     key[r] = e < w1 ? eg_load(keys, ids, add, is64, n, e, V) : 0u;
     eg_wave_step<false>(mine, (key[r] >> sh) & 255u, e < w1, lane, [](int) {});
   }
+  if (wave == 0) {  // exclusive sums of the digits' totals, 4 a lane
+    const int* total = hist + (size_t)256 * gridDim.x + 4 * lane;
+    int a[4], s = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a[k] = s;
+      s += total[k];
+    }
+    int inc = s;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += t;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) low[4 * lane + k] = inc - s + a[k];
+  }
   __syncthreads();
   {
-    int s = hist[(size_t)tid * gridDim.x + blockIdx.x];
+    int s = low[tid] + hist[(size_t)tid * gridDim.x + blockIdx.x];
     for (int w = 0; w < 4; ++w) {
       const int c = cnt[w * 256 + tid];
       cnt[w * 256 + tid] = s;
@@ -363,15 +372,19 @@ __device__ __forceinline__ void eg_sum_entries(float (&acc)[VEC], const int* __r
   }
 }
 
-// Partial sums of the chunks [64 c, 64 c + 64) whose entries share one id (else nothing).
+// Partial sums of the chunks whose EG_CHUNK entries share one id (else nothing).  Behind the
+// last entry of an id of a row, keys holds anything: seg tells.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) embed_chunk_kernel(const uint32_t* __restrict__ keys,
+                                                          const int2* __restrict__ seg,
                                                           const int* __restrict__ ents, const T* __restrict__ dx,
                                                           float* __restrict__ part, int n, int n2, int V, int H) {
   const int ch = blockIdx.x * 4 + (threadIdx.x >> 6), e0 = ch * EG_CHUNK;
   if (e0 + EG_CHUNK > n2) return;
   const uint32_t k = keys[e0];
-  if (k >= (uint32_t)V || keys[e0 + EG_CHUNK - 1] != k) return;
+  if (k >= (uint32_t)V) return;
+  const int2 s = seg[k];
+  if (s.x > e0 || s.y < e0 + EG_CHUNK) return;
   const int c = blockIdx.y * 64 + (threadIdx.x & 63);
   if (c >= H / VEC) return;
   float acc[VEC];
@@ -382,8 +395,9 @@ __global__ void __launch_bounds__(256) embed_chunk_kernel(const uint32_t* __rest
   for (int j = 0; j < VEC; ++j) part[(size_t)ch * H + (size_t)c * VEC + j] = acc[j];
 }
 
-// dE: block b owns rows [4 b, 4 b + 4) x chunks [64 y, 64 y + 64).  A row's terms are its
-// entries up to a chunk border, the sums of its whole chunks, and the entries behind.
+// dE: of B blocks, block b owns the rows b + i B, i = 0..3 (ids of many entries are often
+// neighbours), x chunks [64 y, 64 y + 64).  A row's terms are its entries up to a chunk
+// border, the sums of its whole chunks, and the entries behind.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) embed_rows_kernel(const int2* __restrict__ seg, const int* __restrict__ ents,
                                                          const T* __restrict__ dx, const float* __restrict__ part,
@@ -436,21 +450,21 @@ __global__ void __launch_bounds__(256) embed_rows_kernel(const int2* __restrict_
     for (int j = 0; j < VEC; ++j) o.v[j] = (T)(acc[j] * scale);
     reinterpret_cast<vec*>(dt + (size_t)v * H)[c] = o;
   };
-  const int v0 = blockIdx.x * 4;
+  const int nb = gridDim.x, mine = blockIdx.x + wave * nb;
   int a, b;
-  if (v0 + wave < V) {
-    const int2 s = seg[v0 + wave];
+  if (mine < V) {
+    const int2 s = seg[mine];
     const int nt = terms(s, a, b);
     if (nt <= EG_COOP && on) {
       float acc[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
       sum(acc, s, a, b, 0, nt);
-      store(v0 + wave, acc);
+      store(mine, acc);
     }
   }
-  for (int r = 0; r < 4 && v0 + r < V; ++r) {  // the same for every wave: seg decides
-    const int2 s = seg[v0 + r];
+  for (int v = blockIdx.x; v < V; v += nb) {  // at most 4; the same for every wave: seg decides
+    const int2 s = seg[v];
     const int nt = terms(s, a, b);
     if (nt <= EG_COOP) continue;
     const int per = (nt + 3) / 4;
@@ -464,7 +478,7 @@ __global__ void __launch_bounds__(256) embed_rows_kernel(const int2* __restrict_
     if (wave == 0 && on) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) acc[j] = (red[0][lane][j] + red[1][lane][j]) + (red[2][lane][j] + red[3][lane][j]);
-      store(v0 + r, acc);
+      store(v, acc);
     }
     __syncthreads();
   }
@@ -491,8 +505,8 @@ int eg_backward(const void* ids, const void* add, int is64, const void* dx, void
     return hipGetLastError() == hipSuccess ? 0 : 2;
   }
   const int nchunk = n2 / EG_CHUNK;
-  embed_chunk_kernel<T, VEC><<<dim3((nchunk + 3) / 4, ncb), dim3(256), 0, st>>>(keys, ents, (const T*)dx, part, n, n2,
-                                                                                V, H);
+  embed_chunk_kernel<T, VEC><<<dim3((nchunk + 3) / 4, ncb), dim3(256), 0, st>>>(keys, seg, ents, (const T*)dx, part, n,
+                                                                                n2, V, H);
   embed_rows_kernel<T, VEC><<<dim3((V + 3) / 4, ncb), dim3(256), 0, st>>>(seg, ents, (const T*)dx, part, (T*)dt, n, V,
                                                                           H, scale);
   return hipGetLastError() == hipSuccess ? 0 : 2;
@@ -520,7 +534,7 @@ int sg_embed_fwd(const void* ids, const void* add, int is64, const void* table, 
 int sg_embed_grad_ws(int n2, int V, int H) {
   if (n2 <= EG_SMALL) return 0;
   const long tiles = (n2 + EG_TILE - 1) / EG_TILE;
-  return (int)((2L * V + 4L * n2 + 256 * tiles + (long)(n2 / EG_CHUNK) * H + 63) / 64);
+  return (int)((2L * V + 4L * n2 + 256 * (tiles + 1) + (long)(n2 / EG_CHUNK) * H + 63) / 64);
 }
 
 int sg_embed_grad(const void* ids, const void* add, int is64, const void* dx, void* dt, int n, int V, int H,
@@ -544,21 +558,21 @@ int sg_embed_grad(const void* ids, const void* add, int is64, const void* dx, vo
     int* eb[2] = {w, w + n2};
     w += 2L * n2;
     int* hist = w;
-    w += 256 * tiles;
+    w += 256 * (tiles + 1);
     part = (float*)w;
     int passes = 1;
     while (passes < 4 && (V >> (8 * passes)) != 0) ++passes;
-    if (n2 <= EG_LDS && V < (1 << (32 - EG_IDX_BITS))) {
+    if (n2 <= EG_RANGE && V <= EG_RANGE_V) {
       keys = kb[0];
       ents = eb[0];
-      embed_sort_lds_kernel<<<dim3(1), dim3(1024), 0, st>>>(ids, add, is64, n, n2, V, passes, keys, ents, seg);
+      embed_range_sort_kernel<<<dim3((V + 255) / 256), dim3(1024), 0, st>>>(ids, add, is64, n, n2, V, keys, ents, seg);
     } else {
       const uint32_t* ksrc = nullptr;
       const int* esrc = nullptr;
       for (int p = 0; p < passes; ++p) {
         embed_hist_kernel<<<dim3((unsigned)tiles), dim3(256), 0, st>>>(ksrc, ids, add, is64, n, n2, V, 8 * p, hist,
                                                                        p == 0 ? seg : nullptr);
-        embed_scan_kernel<<<dim3(1), dim3(1024), 0, st>>>(hist, (int)(256 * tiles));
+        embed_scan_kernel<<<dim3(64), dim3(256), 0, st>>>(hist, (int)tiles);
         embed_scatter_kernel<<<dim3((unsigned)tiles), dim3(256), 0, st>>>(ksrc, esrc, ids, add, is64, n, n2, V, 8 * p,
                                                                           hist, kb[p & 1], eb[p & 1]);
         ksrc = kb[p & 1];

@@ -55,9 +55,10 @@ def _check(ids, table, add, scale, seed=0):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n,V,H", [(1, 1, 1), (45, 8192, 256), (128, 300, 65), (129, 5, 8), (257, 77, 96), (4001, 1000, 576),
-                                   (8192, 40, 100), (8193, 8576, 64), (20011, 300000, 24)])
+                                   (8192, 40, 100), (8193, 8576, 64), (20011, 300000, 24),
+                                   (300001, 500, 8)])
 def test_embed_matches_definition(dtype, n, V, H):
-    """Both sides of every rule: one launch / LDS sort / radix passes, one to three 8-bit
+    """Both sides of every rule: one launch / sort by ranges / radix passes, one to three 8-bit
     passes, 16-byte rows and odd ones, with and without a second row."""
     g = torch.Generator(device=dev).manual_seed(n)
     table = torch.randn(V, H, generator=g, device=dev).to(dtype)
@@ -67,7 +68,7 @@ def test_embed_matches_definition(dtype, n, V, H):
     _check(ids.int(), table, add.int(), 3.0 ** 0.5, seed=1)
 
 
-@pytest.mark.parametrize("n", [200, 3000, 40000])
+@pytest.mark.parametrize("n", [200, 3000, 16000, 40000])
 def test_embed_same_id_everywhere(n):
     """One id for every position (and a lone other at each end): the long-run path."""
     table = torch.randn(50, 72, device=dev)
