@@ -38,6 +38,7 @@
 // 2^-24: there P is scaled by 2^8 and dS by a power of two that the largest |do| sets.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 namespace {
 
@@ -59,7 +60,7 @@ __device__ const uint4 at_zero = {0, 0, 0, 0};  // what rows outside a sequence 
 struct AtArgs {
   const uint16_t *q, *k, *v, *o, *dout;
   uint16_t *out, *olo, *dq, *dk, *dv;  // olo: what rounding took from o, or null (no backward)
-  float *lse, *dsum, *part;   // [B, nh, Tp]: L in log2, D; [B, nh, T, D] x 2: dk, dv by query head
+  float *lse, *dsum, *part;   // [B, nh, Tp]: -L in log2, -D; [B, nh, T, D] x 2: dk, dv by query head
   const float* omax;          // fp16: AT_MAXPARTS maxima of |do|
   const int* lens;            // [B] or null
   long qb, qh, qt, kb, kh, kt, vb, vh, vt;  // strides in elements
@@ -252,9 +253,11 @@ __global__ void __launch_bounds__(NW * 64) attn_fwd_kernel(AtArgs a) {
         for (int r = 0; r < 16; ++r)
           if (k0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h >= lim) s[u][r] = -INFINITY;
     }
-    float top = fmaxf(s[0][0], s[1][0]);
+    // (NaN passes: then m, l and o are NaN too)
+    float top = __builtin_elementwise_maximum(s[0][0], s[1][0]);
 #pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
+    for (int r = 1; r < 16; ++r)
+      top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][r]), s[1][r]);
     top = at_max_halves(top) * c;
     // any reference value serves the softmax: m follows the maximum only when it rises by
     // over 2^8, so most tiles skip the rescaling of o
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(NW * 64) attn_fwd_kernel(AtArgs a) {
       }
     }
   }
-  if (h == 0 && qr < a.Tp) a.lse[(size_t)bh * a.Tp + qr] = on ? m + __log2f(l) : INFINITY;
+  if (h == 0 && qr < a.Tp) a.lse[(size_t)bh * a.Tp + qr] = on ? -(m + __log2f(l)) : -INFINITY;
 }
 
 // fp16: the factor on dS, 16 / 2^floor(log2 max|do|)
@@ -371,21 +374,17 @@ __global__ void __launch_bounds__(NW * 64) attn_dq_kernel(AtArgs a) {
         dsum = fmaf(at_float<BF>(of[s][j]) + at_float<BF>(lo[s][j]), at_float<BF>(df[s][j]), dsum);
   }
   dsum = at_sum_halves(dsum);
-  if (h == 0 && qr < a.Tp) a.dsum[(size_t)bh * a.Tp + qr] = dsum;
-  const float lse = on ? a.lse[(size_t)bh * a.Tp + qr] : INFINITY;
+  if (h == 0 && qr < a.Tp) a.dsum[(size_t)bh * a.Tp + qr] = -dsum;
+  const float lse = on ? a.lse[(size_t)bh * a.Tp + qr] : -INFINITY;  // -L
   const float c = a.scale * AT_LOG2E;
   float dsf = 1.f;
   if constexpr (!BF) dsf = at_ds_factor(a.omax, lane);
   f32x16 dq[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) dq[dt] = (f32x16)0.f;
-  for (int t = 0; t < nt; ++t) {
-    at_wait();
-    if (t + 1 < nt) stage(t + 1);
-    const int k0 = t * AT_KT;
-    if (k0 >= kw) continue;
-    const uint16_t *ks = sm + (t & 1) * 2 * TILE, *vs = ks + TILE;
-    const bool border = k0 + AT_KT > (a.causal ? min(len, qw + 1) : len);
+  // BORDER: some lane's border of keys is in the tile
+  auto tile = [&](const uint16_t* ks, int k0, auto border) {
+    const uint16_t* vs = ks + TILE;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 s = (f32x16)0.f, dp = (f32x16)(-dsum);
@@ -396,8 +395,8 @@ __global__ void __launch_bounds__(NW * 64) attn_dq_kernel(AtArgs a) {
       float ds[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
-        if (border && k0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h >= lim) p = 0.f;
+        float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, lse));
+        if (border.value && k0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h >= lim) p = 0.f;
         ds[r] = BF ? p * dp[r] : p * dp[r] * dsf;
       }
 #pragma unroll
@@ -408,6 +407,17 @@ __global__ void __launch_bounds__(NW * 64) attn_dq_kernel(AtArgs a) {
           dq[dt] = at_mma<BF>(at_col<D>(ks, 32 * u + 16 * e, dt, lane), pf, dq[dt]);
       }
     }
+  };
+  const int whole = a.causal ? min(len, qw + 1) : len;  // keys that every lane of the wave sees
+  for (int t = 0; t < nt; ++t) {
+    at_wait();
+    if (t + 1 < nt) stage(t + 1);
+    const int k0 = t * AT_KT;
+    const uint16_t* ks = sm + (t & 1) * 2 * TILE;
+    if (k0 + AT_KT <= whole)
+      tile(ks, k0, std::false_type());
+    else if (k0 < kw)
+      tile(ks, k0, std::true_type());
   }
   if (qr < a.T) {
     uint16_t* row = a.dq + ((size_t)bh * a.T + qr) * D;
@@ -458,14 +468,10 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = (f32x16)0.f;
-  for (int i = 0; i < nt; ++i) {
-    at_wait();
-    if (i + 1 < nt) stage(i + 1);
-    const int q0 = (t0 + i % per) * AT_KT;
-    if (kw >= len || (a.causal && q0 + AT_KT <= kw)) continue;
-    const uint16_t *qs = sm + (i & 1) * STAGE, *os = qs + TILE;
-    const float* ls = reinterpret_cast<const float*>(os + TILE);
-    const bool border = a.causal && q0 < kw + 31;
+  // BORDER: the tile holds queries before some lane's key
+  auto tile = [&](const uint16_t* qs, int q0, auto border) {
+    const uint16_t* os = qs + TILE;
+    const float* ls = reinterpret_cast<const float*>(os + TILE);  // -L, -D
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 s = (f32x16)0.f, dp;
@@ -475,7 +481,7 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
         const float4 x = *reinterpret_cast<const float4*>(ls + 32 * u + 8 * e + 4 * h);
         const float4 y = *reinterpret_cast<const float4*>(ls + AT_KT + 32 * u + 8 * e + 4 * h);
         lq[4 * e] = x.x, lq[4 * e + 1] = x.y, lq[4 * e + 2] = x.z, lq[4 * e + 3] = x.w;
-        dp[4 * e] = -y.x, dp[4 * e + 1] = -y.y, dp[4 * e + 2] = -y.z, dp[4 * e + 3] = -y.w;
+        dp[4 * e] = y.x, dp[4 * e + 1] = y.y, dp[4 * e + 2] = y.z, dp[4 * e + 3] = y.w;
       }
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) s = at_mma<BF>(at_row<D>(qs, 32 * u + (lane & 31), e, h), kf[e], s);
@@ -484,8 +490,8 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
       float p[16], ds[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, (BF ? 0.f : (float)AT_FP16_P) - lq[r]));
-        if (border && q0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h < kr) p[r] = 0.f;
+        p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, BF ? lq[r] : lq[r] + (float)AT_FP16_P));
+        if (border.value && q0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h < kr) p[r] = 0.f;
         ds[r] = BF ? p[r] * dp[r] : p[r] * dp[r] * dsf;
       }
 #pragma unroll
@@ -498,6 +504,17 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
         }
       }
     }
+  };
+  for (int i = 0; i < nt; ++i) {
+    at_wait();
+    if (i + 1 < nt) stage(i + 1);
+    const int q0 = (t0 + i % per) * AT_KT;
+    const uint16_t* qs = sm + (i & 1) * STAGE;
+    if (kw >= len) continue;
+    if (!a.causal || q0 >= kw + 31)
+      tile(qs, q0, std::false_type());
+    else if (q0 + AT_KT > kw)
+      tile(qs, q0, std::true_type());
   }
   if (kr >= a.T) return;
   const float fk = BF ? a.scale : a.scale / (dsf * (1 << AT_FP16_P));
