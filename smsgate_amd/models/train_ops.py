@@ -379,30 +379,31 @@ class _LmLoss(torch.autograd.Function):
         V, H = table.shape
         N, dev, fp16, is64 = labels.numel(), h.get_device(), int(h.dtype == torch.float16), int(
             labels.dtype == torch.int64)
-        h, table, labels = _aligned(h), _aligned(table), labels.contiguous()
+        shape, h, table, labels = h.shape, _aligned(h), _aligned(table), labels.contiguous()
         lib = _lib()
-        plan = (ctypes.c_int * 5)()
+        plan = (ctypes.c_int * 6)()
         _ok(lib.sg_loss_plan(N, V, H, plan), "loss_plan")
-        hc = h.new_empty(plan[0], plan[1])
-        state = torch.empty(plan[2] * 64, dtype=torch.int32, device=h.device)
-        ws = torch.empty(plan[3] * 64, dtype=torch.float32, device=h.device)
+        # the labelled rows and the table as the products read them, kept for the backward
+        hc, ec = h.new_empty(plan[0], plan[1]), h.new_empty(plan[2], plan[1])
+        state = torch.empty(plan[3] * 64, dtype=torch.int32, device=h.device)
+        ws = torch.empty(plan[4] * 64, dtype=torch.float32, device=h.device)
         loss = torch.empty(labels.shape if mode == 2 else (), dtype=torch.float32, device=h.device)
         _run(dev, "loss_fwd", lib.sg_loss_fwd, h.data_ptr(), table.data_ptr(), labels.data_ptr(), is64, ignore,
-             hc.data_ptr(), state.data_ptr(), ws.data_ptr(), loss.data_ptr(), N, V, H, mode, fp16)
-        ctx.save_for_backward(hc, table, state)
-        ctx.plan = (lib.sg_loss_bwd, dev, h.shape, (N, V, H, mode, fp16), plan[4] * 64)
+             hc.data_ptr(), ec.data_ptr(), state.data_ptr(), ws.data_ptr(), loss.data_ptr(), N, V, H, mode, fp16)
+        ctx.save_for_backward(hc, ec, state)
+        ctx.plan = (lib.sg_loss_bwd, dev, shape, (N, V, H, mode, fp16), plan[5] * 64)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        hc, table, state = ctx.saved_tensors
+        hc, ec, state = ctx.saved_tensors
         fn, dev, shape, dims, words = ctx.plan
         g = g.contiguous()
         dh = hc.new_empty(shape) if ctx.needs_input_grad[0] else None
-        dt = torch.empty_like(table) if ctx.needs_input_grad[1] else None
+        dt = hc.new_empty(dims[1], dims[2]) if ctx.needs_input_grad[1] else None
         ws = g.new_empty(words)
-        _run(dev, "loss_bwd", fn, hc.data_ptr(), table.data_ptr(), state.data_ptr(), g.data_ptr(), ws.data_ptr(),
+        _run(dev, "loss_bwd", fn, hc.data_ptr(), ec.data_ptr(), state.data_ptr(), g.data_ptr(), ws.data_ptr(),
              ops._p(dh), ops._p(dt), *dims)
         return dh, dt, None, None, None
 

@@ -176,7 +176,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         fn.restype = _c_int
     # vocabulary cross entropy and its gradients (csrc/loss_kernels.hip)
     lib.sg_loss_plan.argtypes = [_c_int] * 3 + [_vp]
-    lib.sg_loss_fwd.argtypes = [_vp] * 3 + [_c_int] * 2 + [_vp] * 4 + [_c_int] * 5 + [_vp]
+    lib.sg_loss_fwd.argtypes = [_vp] * 3 + [_c_int] * 2 + [_vp] * 5 + [_c_int] * 5 + [_vp]
     lib.sg_loss_bwd.argtypes = [_vp] * 7 + [_c_int] * 5 + [_vp]
     for fn in (lib.sg_loss_plan, lib.sg_loss_fwd, lib.sg_loss_bwd):
         fn.restype = _c_int

@@ -53,14 +53,14 @@ constexpr float LK_FP16 = 1024.f;  // factor on d in fp16
 struct LossArgs {
   const uint16_t *h, *table;
   const void* labels;
-  uint16_t *hc, *d, *dh, *dtable;
+  uint16_t *hc, *ec, *d, *dh, *dtable;  // hc, ec, d: panels
   int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; [1]
   float *lse, *rl, *loss, *w;       // [Mp] L in log2; [Mp] loss; out; [Mp] row weights or null
   float2* part;                     // [v tiles][Mp] (maximum, sum of exp(z - maximum))
   float* share;                     // [splits][Mp][Hp]
   const float *g, *gmax;            // incoming gradient; none: its largest magnitude
   long ignore;
-  int N, V, H, Mp, Hp, is64, mode;  // mode 0 mean, 1 sum, 2 none
+  int N, V, H, Mp, Hp, Vp, is64, mode;  // mode 0 mean, 1 sum, 2 none
   int v0, vn;                       // piece: first row, rows (of them < V - v0 real)
   int splits, want, most, first;    // dh: shares of Mp rows in the workspace; blocks wanted; splits at most
   int bl, nr;                       // dh: rows of a tile, tiles over H
@@ -126,65 +126,46 @@ __device__ __forceinline__ float4 lk_four(const f32x16& x, int e, float f) {
   return make_float4(x[4 * e] * f, x[4 * e + 1] * f, x[4 * e + 2] * f, x[4 * e + 3] * f);
 }
 
-// What is XORed into the 16-byte chunk index of tile row `row`, for rows of CPR chunks.  LDS
-// serves 256 bytes a cycle over 64 banks: 16 lanes of a row read (16 rows, one chunk) or 32
-// of a transposing read (4 rows, 4 chunks), each conflict-free if those chunks differ modulo
-// 256 bytes.
-template <int CPR>
-__device__ __forceinline__ int lk_swz(int row) {
-  if constexpr (CPR == 4)  // 64-byte rows: row & 3 is a quarter of the banks already
-    return (row >> 2) & 3;
-  else if constexpr (CPR == 8)  // 128-byte rows: row & 1 is half of the banks already
-    return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) | ((row >> 3) & 1) << 1;
-  else if constexpr (CPR % 16 == 0)
-    return (row & 3) << 2;
-  else {
-    static_assert(CPR % 16 == 8, "rows of whole 128 bytes");
-    return ((row >> 1) & 1) << 2;
-  }
-}
-
 // ---- rows with a label -----------------------------------------------------------------
 // One block: places of the labelled rows, in order.  A label outside [0, V) becomes -2 (its
 // loss and gradients are NaN).
 __global__ void __launch_bounds__(1024) loss_rows_kernel(LossArgs a) {
   __shared__ int part[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const unsigned long long before = (1ull << lane) - 1;
   int base = 0;
-  for (int i0 = 0; i0 < a.N; i0 += 8192) {
-    long y[8];
+  for (int i0 = 0; i0 < a.N; i0 += 16384) {  // a wave owns 1024 labels, 64 at a time
+    const int w0 = i0 + 1024 * wave + lane;
+    long y[16];
     int n = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = i0 + 8 * tid + k;
+    for (int k = 0; k < 16; ++k) {
+      const int i = w0 + 64 * k;
       y[k] = i < a.N ? (a.is64 ? reinterpret_cast<const long*>(a.labels)[i]
                                : (long)reinterpret_cast<const int*>(a.labels)[i])
                      : a.ignore;
-      n += y[k] != a.ignore;
     }
-    int inc = n;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += t;
-    }
-    if (lane == 63) part[wave] = inc;
+    for (int k = 0; k < 16; ++k) n += __popcll(__ballot(y[k] != a.ignore));
+    if (lane == 0) part[wave] = n;
     __syncthreads();
-    int at = base + inc - n, all = 0;
+    int at = base, all = 0;
     for (int w = 0; w < 16; ++w) {
       if (w < wave) at += part[w];
       all += part[w];
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = i0 + 8 * tid + k;
-      if (i >= a.N) continue;
+    for (int k = 0; k < 16; ++k) {
+      const int i = w0 + 64 * k;
       const bool on = y[k] != a.ignore;
-      a.pos[i] = on ? at : -1;
+      const unsigned long long m = __ballot(on);
+      const int place = at + __popcll(m & before);
+      at += __popcll(m);
+      if (i >= a.N) continue;
+      a.pos[i] = on ? place : -1;
       if (on) {
-        a.rows[at] = i;
-        a.lab[at] = y[k] >= 0 && y[k] < a.V ? (int)y[k] : -2;
-        ++at;
+        a.rows[place] = i;
+        a.lab[place] = y[k] >= 0 && y[k] < a.V ? (int)y[k] : -2;
       } else if (a.mode == 2) {
         a.loss[i] = 0.f;
       }
@@ -195,88 +176,74 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(LossArgs a) {
   if (tid == 0) a.cnt[0] = base;
 }
 
-// hc[m] = h[rows[m]], zeros behind the last row (up to a whole tile) and column; 16 bytes a thread
-__global__ void __launch_bounds__(256) loss_gather_kernel(LossArgs a) {
+// Every operand of the products lies in panels of LK_PANEL columns, [panel][rows][LK_PANEL]:
+// a tile is runs of memory of 1 KB and more whichever way it is read, nothing of it is out of
+// bounds, and its copies need no address but a wave's own.  (Tiles of the matrices as they
+// come, 64 bytes a row, kept the copies waiting for twice as many memory requests.)
+constexpr int LK_PANEL = 32;
+__device__ __forceinline__ size_t lk_at(long rows, long row, int c) {  // 16-byte chunk c of a row
+  return ((c >> 2) * rows + row) * LK_PANEL + (c & 3) * 8;
+}
+
+// hc = h[rows] (zeros behind the last row, up to a whole tile, and column) and ec = E, in
+// panels; 16 bytes a thread
+__global__ void __launch_bounds__(256) loss_layout_kernel(LossArgs a) {
   const int nch = a.Hp / 8, cnt = a.cnt[0];
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const int m = (int)(i / nch), c = (int)(i - (long)m * nch);
-  if (m >= (cnt + LK_PAD - 1) / LK_PAD * LK_PAD || m >= a.Mp) return;
+  const long r = i / nch;
+  const int c = (int)(i - r * nch);
   uint4 v = make_uint4(0, 0, 0, 0);
+  if (r < a.Vp) {
+    if (r < a.V && 8 * c < a.H) v = *reinterpret_cast<const uint4*>(a.table + (size_t)r * a.H + 8 * c);
+    *reinterpret_cast<uint4*>(a.ec + lk_at(a.Vp, r, c)) = v;
+    return;
+  }
+  const int m = (int)(r - a.Vp);
+  if (m >= (cnt + LK_PAD - 1) / LK_PAD * LK_PAD || m >= a.Mp) return;
   if (m < cnt && 8 * c < a.H) v = *reinterpret_cast<const uint4*>(a.h + (size_t)a.rows[m] * a.H + 8 * c);
-  *reinterpret_cast<uint4*>(a.hc + (size_t)m * a.Hp + 8 * c) = v;
+  *reinterpret_cast<uint4*>(a.hc + lk_at(a.Mp, m, c)) = v;
 }
 
 // ---- products --------------------------------------------------------------------------
-// Row operand: row `row` of a [rows][BK] tile, k-values 16 s + 8 h + 0..7.
-template <int BK>
+// A tile in LDS is [panel][rows][32] too, each 16-byte chunk XORed by its row: LDS serves 256
+// bytes a cycle over 64 banks, and neither 16 lanes of a row read (16 rows, one chunk) nor
+// 32 of a transposing read (4 rows, 4 chunks) meet on a bank.
+__device__ __forceinline__ int lk_swz(int row) { return (row >> 2) & 3; }
+
+// Row operand: row `row`, k-values (columns of the tile's panel) 16 s + 8 h + 0..7.
 __device__ __forceinline__ u16x8 lk_row(const uint16_t* tile, int row, int s, int h) {
-  return *reinterpret_cast<const u16x8*>(tile + row * BK + (((2 * s + h) ^ lk_swz<BK / 8>(row)) << 3));
+  return *reinterpret_cast<const u16x8*>(tile + row * LK_PANEL + (((2 * s + h) ^ lk_swz(row)) << 3));
 }
 
-// Column operand: column c0 + (lane & 31) of a [BK][COLS] tile, the same k-values (its rows).
-template <int COLS>
-__device__ __forceinline__ u16x8 lk_col(const uint16_t* tile, int c0, int s, int lane) {
-  const int i = lane & 15, ch = (c0 >> 3) + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+// Column operand: column lane & 31 of a panel, the same k-values (its 32 rows).
+__device__ __forceinline__ u16x8 lk_col(const uint16_t* panel, int s, int lane) {
+  const int i = lane & 15, ch = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
   const int row = 16 * s + 8 * (lane >> 5) + (i >> 2);
   const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lk_tr_t)(tile + row * COLS + ((ch ^ lk_swz<COLS / 8>(row)) << 3) + ((i & 1) << 2)));
+      (lk_tr_t)(panel + row * LK_PANEL + ((ch ^ lk_swz(row)) << 3) + ((i & 1) << 2)));
   const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lk_tr_t)(tile + (row + 4) * COLS + ((ch ^ lk_swz<COLS / 8>(row + 4)) << 3) + ((i & 1) << 2)));
+      (lk_tr_t)(panel + (row + 4) * LK_PANEL + ((ch ^ lk_swz(row + 4)) << 3) + ((i & 1) << 2)));
   const s16x4 both[2] = {lo, hi};
   u16x8 r;
   __builtin_memcpy(&r, both, 16);
   return r;
 }
 
-// Copies a [rows r0 ..][BK k] or (COL) [BK k][columns r0 ..] tile of SIDE rows or columns by
-// DMA.  Nothing outside the matrix is read: rows or columns from `rend` on repeat the last
-// one (their results are masked or not stored), k-values from the `rem`-th on another of the
-// same row or column (the other operand holds zeros there; rem >= 1).  Offsets of 32 bits
-// from a base that is the same for the wave: a step costs one scalar addition and the copies
-// themselves.
-template <int SIDE, int NW, bool COL, int BK>
-struct LkStage {
-  static constexpr int CPR = COL ? SIDE / 8 : BK / 8;  // chunks a tile row
-  static constexpr int N = SIDE * BK / 512 / NW;       // DMA instructions a wave
-  static_assert(SIDE * BK % (512 * NW) == 0, "whole instructions a wave");
-  const char* base;
-  uint32_t off[N];
-  int ld;  // bytes
-  __device__ __forceinline__ static int chunk(int i, int wave, int lane, int& row) {
-    const int q = (wave + NW * i) * 64 + lane;
-    row = q / CPR;
-    return (q % CPR) ^ lk_swz<CPR>(row);
-  }
-  __device__ __forceinline__ void init(const uint16_t* src, int ld_, int r0, int rend, int wave, int lane) {
-    ld = 2 * ld_;
-    const int rb = COL ? min(r0, rend - 8) : min(r0, rend - 1);
-    base = reinterpret_cast<const char*>(src) + (COL ? 2 * (long)rb : (long)rb * ld);
+// Copies a tile by DMA, 16 rows of a panel an instruction.  !COL: SIDE rows of one panel;
+// COL: 32 rows of SIDE / 32 panels, `stride` elements apart (panels behind the last repeat
+// it: their results are not stored).  src: the tile's first row and panel.
+template <int SIDE, int NW, bool COL>
+__device__ __forceinline__ void lk_stage(const uint16_t* src, long stride, int panels, uint16_t* dst, int wave,
+                                         uint32_t lane_off) {
+  static_assert(SIDE / 16 % NW == 0, "whole instructions a wave");
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      int row;
-      const int c = chunk(i, wave, lane, row);
-      off[i] = COL ? (uint32_t)(row * ld + 2 * (min(r0 + 8 * c, rend - 8) - rb))
-                   : (uint32_t)((min(r0 + row, rend - 1) - rb) * ld + 16 * c);
-    }
+  for (int i = 0; i < SIDE / 16 / NW; ++i) {
+    const int g = wave + NW * i;
+    const uint16_t* p = src + (COL ? min(g >> 1, panels - 1) * stride + (g & 1) * 512 : g * 512);
+    __builtin_amdgcn_global_load_lds((const void*)(reinterpret_cast<const char*>(p) + lane_off),
+                                     (lk_lds_t)(dst + g * 512), 16, 0, 0);
   }
-  // at: byte offset of the step's first k-value
-  __device__ __forceinline__ void issue(uint16_t* dst, long at, int rem, int wave, int lane) const {
-    const char* p = base + at;
-    if (rem >= BK) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        __builtin_amdgcn_global_load_lds((const void*)(p + off[i]), (lk_lds_t)(dst + (wave + NW * i) * 512), 16, 0, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        int row;
-        const int c = chunk(i, wave, lane, row), over = (COL ? row : 8 * c) - (rem - 1);
-        const uint32_t o = off[i] - (over <= 0 ? 0u : (uint32_t)(COL ? over * ld : 16 * c));
-        __builtin_amdgcn_global_load_lds((const void*)(p + o), (lk_lds_t)(dst + (wave + NW * i) * 512), 16, 0, 0);
-      }
-    }
-  }
-};
+}
 
 // Splits of the piece's columns that dh's share is taken in, for `tiles` tiles over `rows`
 // rows: enough blocks for the card, as many as the workspace holds.  The same for every
@@ -287,22 +254,16 @@ __device__ __forceinline__ int lk_splits(int rows, int tiles, const LossArgs& a)
   return max(1, min(min(fit, want), a.most));
 }
 
-// d lies in panels of LK_PANEL columns, [panel][Mp][LK_PANEL]: a tile of it is one run of
-// memory whichever way it is read (rows of the whole piece, 32 KB apart, cost 2 us a step).
-constexpr int LK_PANEL = 256;
-
 // MODE 0 / 1: lane side = hidden rows, register side = vocabulary rows, k = H.
 // MODE 2: lane = the piece's vocabulary rows, register = H, k = hidden rows.
 // MODE 3: lane = hidden rows, register = H, k = a split of the piece.
-// BK k-values a step, ST buffers: the copies of the next ST - 1 steps are in flight.
-template <bool BF, int MODE, int BL, int BR, int WL, int WR, int BK, int ST>
+// 32 k-values a step, ST buffers: the copies of the next ST - 1 steps are in flight.
+template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST>
 __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   constexpr int NW = WL * WR, TL = BL / WL, TR = BR / WR, FL = TL / 32, FR = TR / 32;
   constexpr bool LCOL = MODE == 2, RCOL = MODE >= 2;
-  constexpr int STAGE = (BL + BR) * BK;
+  constexpr int BK = LK_PANEL, STAGE = (BL + BR) * BK, NI = (BL + BR) / 16 / NW;
   static_assert(ST * STAGE * 2 <= 160 * 1024 && BL % (32 * WL) == 0 && BR % (32 * WR) == 0, "tile");
-  static_assert(LK_PANEL % BL == 0 || MODE != 2, "d's columns of a tile lie in one panel");
-  static_assert(LK_PANEL % BR == 0 || MODE != 1, "d's columns of a tile lie in one panel");
   __shared__ __attribute__((aligned(16))) uint16_t sm[ST * STAGE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int wl = wave / WR, wr = wave % WR;
@@ -325,39 +286,30 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   }
   const int band = t / (8 * nr), bl = t - band * 8 * nr, bw = min(8, nl - 8 * band);
   const int l0 = (8 * band + bl % bw) * BL, r0 = (bl / bw) * BR;
-  int kb = 0, ke = (a.H + BK - 1) / BK * BK;
+  int kb = 0, ke = (a.H + BK - 1) / BK * BK;  // (a step wholly behind either matrix would add zeros)
   if constexpr (MODE == 2) ke = (cnt + BK - 1) / BK * BK;
   if constexpr (MODE == 3) {
     const int per = (a.vn / LK_K + splits - 1) / splits * LK_K;
-    // steps wholly behind the vocabulary are left out: d is zero there, and E has no such rows
     const int end = (min(a.vn, a.V - a.v0) + BK - 1) / BK * BK;
     kb = min(end, z * per);
     ke = min(end, kb + per);
   }
-  LkStage<BL, NW, LCOL, BK> sl;
-  LkStage<BR, NW, RCOL, BK> sr;
-  const long panel = (long)a.Mp * LK_PANEL;
-  if constexpr (MODE <= 1) {
-    sl.init(a.hc, a.Hp, l0, a.Mp, wave, lane);
-    sr.init(a.table, a.H, a.v0 + r0, a.V, wave, lane);
-  } else if constexpr (MODE == 2) {
-    sl.init(a.d + l0 / LK_PANEL * panel, LK_PANEL, l0 % LK_PANEL, LK_PANEL, wave, lane);
-    sr.init(a.hc, a.Hp, r0, a.Hp, wave, lane);
-  } else {
-    sl.init(a.d, LK_PANEL, l0, a.Mp, wave, lane);
-    sr.init(a.table + (size_t)a.v0 * a.H, a.H, r0, a.H, wave, lane);
-  }
+  const uint32_t lane_off = (lane >> 2) * 64 + (((lane & 3) ^ lk_swz(lane >> 2)) << 4);
+  const long mpan = (long)a.Mp * LK_PANEL, vpan = (long)a.Vp * LK_PANEL;  // a panel of hc or d, of ec
   auto stage = [&](int k0, int buf) {
     uint16_t *ls = sm + buf * STAGE, *rs = ls + BL * BK;
+    const int kp = k0 / LK_PANEL;
     if constexpr (MODE <= 1) {
-      sl.issue(ls, 2 * k0, BK, wave, lane);
-      sr.issue(rs, 2 * k0, a.H - k0, wave, lane);
+      lk_stage<BL, NW, false>(a.hc + kp * mpan + (long)l0 * LK_PANEL, 0, 0, ls, wave, lane_off);
+      lk_stage<BR, NW, false>(a.ec + kp * vpan + (long)(a.v0 + r0) * LK_PANEL, 0, 0, rs, wave, lane_off);
     } else if constexpr (MODE == 2) {
-      sl.issue(ls, (long)k0 * (2 * LK_PANEL), BK, wave, lane);
-      sr.issue(rs, (long)k0 * (2 * a.Hp), BK, wave, lane);
+      lk_stage<BL, NW, true>(a.d + l0 / LK_PANEL * mpan + (long)k0 * LK_PANEL, mpan, BL / 32, ls, wave, lane_off);
+      lk_stage<BR, NW, true>(a.hc + r0 / LK_PANEL * mpan + (long)k0 * LK_PANEL, mpan, (a.Hp - r0) / LK_PANEL, rs, wave,
+                             lane_off);
     } else {
-      sl.issue(ls, 2 * (k0 / LK_PANEL * panel + k0 % LK_PANEL), BK, wave, lane);
-      sr.issue(rs, (long)k0 * (2 * a.H), a.V - a.v0 - k0, wave, lane);
+      lk_stage<BL, NW, false>(a.d + kp * mpan + (long)l0 * LK_PANEL, 0, 0, ls, wave, lane_off);
+      lk_stage<BR, NW, true>(a.ec + r0 / LK_PANEL * vpan + (long)(a.v0 + k0) * LK_PANEL, vpan, (a.Hp - r0) / LK_PANEL,
+                             rs, wave, lane_off);
     }
   };
   f32x16 acc[FR][FL];
@@ -373,7 +325,7 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
     // this wave's copies for this step have landed (those of the ST - 2 steps behind may be
     // under way) and its reads of the buffer before are done; then every wave's
     if (k0 + (ST - 2) * BK < ke)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((decltype(sl)::N + decltype(sr)::N) * (ST - 2)) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NI * (ST - 2)) : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -386,12 +338,12 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
     auto read = [&](int s) {
 #pragma unroll
       for (int j = 0; j < FL; ++j)
-        lf[s & 1][j] =
-            LCOL ? lk_col<BL>(ls, wl * TL + 32 * j, s, lane) : lk_row<BK>(ls, wl * TL + 32 * j + (lane & 31), s, h);
+        lf[s & 1][j] = LCOL ? lk_col(ls + (wl * FL + j) * 32 * LK_PANEL, s, lane)
+                            : lk_row(ls, wl * TL + 32 * j + (lane & 31), s, h);
 #pragma unroll
       for (int i = 0; i < FR; ++i)
-        rf[s & 1][i] =
-            RCOL ? lk_col<BR>(rs, wr * TR + 32 * i, s, lane) : lk_row<BK>(rs, wr * TR + 32 * i + (lane & 31), s, h);
+        rf[s & 1][i] = RCOL ? lk_col(rs + (wr * FR + i) * 32 * LK_PANEL, s, lane)
+                            : lk_row(rs, wr * TR + 32 * i + (lane & 31), s, h);
     };
     read(0);
 #pragma unroll
@@ -450,7 +402,7 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
       const float w = (a.w != nullptr && n < cnt ? a.w[n] : 1.f) * (BF ? 1.f : LK_FP16);
       const int y = (n < cnt ? a.lab[n] : -1) - a.v0 - rn;  // its place in this lane's registers
       const bool here = y >= 0 && y < TR;
-      uint16_t* row = a.d + r0 / LK_PANEL * panel + (size_t)n * LK_PANEL + (r0 % LK_PANEL + wr * TR);
+      uint16_t* row = a.d + (r0 + wr * TR) / LK_PANEL * mpan + (size_t)n * LK_PANEL;
 #pragma unroll
       for (int i = 0; i < FR; ++i) {
 #pragma unroll
@@ -467,7 +419,7 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 4; e += 2)
-          *reinterpret_cast<uint4*>(row + 32 * i + 8 * (e + h)) =
+          *reinterpret_cast<uint4*>(row + i * mpan + 8 * (e + h)) =
               lk_trade<BF>(lk_four(acc[i][j], e, w), lk_four(acc[i][j], e + 1, w));
       }
     }
@@ -504,64 +456,74 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
 }
 
 // ---- joins -----------------------------------------------------------------------------
-// 64 rows a block: L from the tiles' (maximum, sum), the label's logit, the loss.
+// 16 rows a block: L from the tiles' (maximum, sum), the label's logit, the loss.
 template <bool BF>
 __global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
-  __shared__ float2 red[4][64];
-  __shared__ float zy[64];
+  __shared__ float2 red[16][16];
+  __shared__ float zy[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = blockIdx.x * 64, cnt = a.cnt[0];
+  const int m0 = blockIdx.x * 16, cnt = a.cnt[0];
   if (m0 >= cnt) return;
-  const int m = m0 + lane;
+  const int r = threadIdx.x & 15, g = threadIdx.x >> 4;  // row, share of the tiles
   float2 x = make_float2(-INFINITY, 0.f);
-  for (int t = wave; t < tiles; t += 32) {
-    float2 y[8];
+  for (int t = g; t < tiles; t += 64) {
+    float2 y[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 4; ++k) {
       y[k] = make_float2(-INFINITY, 0.f);
-      if (t + 4 * k < tiles) y[k] = a.part[(size_t)(t + 4 * k) * a.Mp + m];
+      if (t + 16 * k < tiles) y[k] = a.part[(size_t)(t + 16 * k) * a.Mp + m0 + r];
     }
     float top = x.x;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = fmaxf(top, y[k].x);
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, y[k].x);
     const float ref = top == -INFINITY ? 0.f : top;
     float s = x.y * lk_exp(x.x - ref);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += y[k].y * lk_exp(y[k].x - ref);
+    for (int k = 0; k < 4; ++k) s += y[k].y * lk_exp(y[k].x - ref);
     x = make_float2(top, s);
   }
-  red[wave][lane] = x;
-  for (int i = wave; i < 64; i += 4) {  // z[y]: a wave a row
-    const int y = m0 + i < cnt ? a.lab[m0 + i] : -1;
-    float s = 0.f;
-    if (y >= 0) {
-      const u16x8* hr = reinterpret_cast<const u16x8*>(a.hc + (size_t)(m0 + i) * a.Hp);
-      const u16x8* er = reinterpret_cast<const u16x8*>(a.table + (size_t)y * a.H);
-      for (int c = lane; c < a.H / 8; c += 64) {
-        const u16x8 p = hr[c], q = er[c];
+  red[g][r] = x;
+  {  // z[y]: 4 rows a wave
+    const u16x8 *hr[4], *er[4];
+    float s[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s = fmaf(lk_float<BF>(p[k]), lk_float<BF>(q[k]), s);
+    for (int k = 0; k < 4; ++k) {
+      const int m = min(m0 + 4 * wave + k, cnt - 1);
+      hr[k] = reinterpret_cast<const u16x8*>(a.h + (size_t)a.rows[m] * a.H);
+      er[k] = reinterpret_cast<const u16x8*>(a.table + (size_t)max(a.lab[m], 0) * a.H);
+      s[k] = 0.f;
+    }
+    for (int c = lane; c < a.H / 8; c += 64) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u16x8 p = hr[k][c], q = er[k][c];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[k] = fmaf(lk_float<BF>(p[e]), lk_float<BF>(q[e]), s[k]);
       }
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (lane == 0) zy[i] = s;
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) s[k] += __shfl_xor(s[k], o, 64);
+      if (lane == 0) zy[4 * wave + k] = s[k];
+    }
   }
   __syncthreads();
-  if (wave != 0) return;
-  float top = fmaxf(fmaxf(red[0][lane].x, red[1][lane].x), fmaxf(red[2][lane].x, red[3][lane].x));
+  const int m = m0 + threadIdx.x;
+  if (threadIdx.x >= 16 || m >= cnt) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) top = fmaxf(top, red[w][threadIdx.x].x);
   const float ref = top == -INFINITY ? 0.f : top;
   float s = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) s += red[w][lane].y * lk_exp(red[w][lane].x - ref);
+  for (int w = 0; w < 16; ++w) s += red[w][threadIdx.x].y * lk_exp(red[w][threadIdx.x].x - ref);
   float ls = __logf(s);
-  if (m < cnt) {
-    if (a.lab[m] == -2) ls = __builtin_nanf("");
-    const float loss = (top - zy[lane]) + ls;
-    a.lse[m] = (top + ls) * LK_LOG2E;
-    a.rl[m] = loss;
-    if (a.mode == 2) a.loss[a.rows[m]] = loss;
-  }
+  if (a.lab[m] == -2) ls = __builtin_nanf("");
+  const float loss = (top - zy[threadIdx.x]) + ls;
+  a.lse[m] = (top + ls) * LK_LOG2E;
+  a.rl[m] = loss;
+  if (a.mode == 2) a.loss[a.rows[m]] = loss;
 }
 
 __device__ __forceinline__ float lk_block_sum(float s, float* red) {
@@ -667,23 +629,23 @@ template <bool BF, int MODE>
 void lk_gemm(const LossArgs& a, const LossPlan& p, hipStream_t st) {
   if (p.small) {
     const int nl = (MODE == 2 ? a.vn : a.Mp) / 64, nr = MODE >= 2 ? (a.H + 63) / 64 : a.vn / 64;
-    loss_gemm_kernel<BF, MODE, 64, 64, 2, 2, 64, 2><<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
+    loss_gemm_kernel<BF, MODE, 64, 64, 2, 2, 4><<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
   } else if constexpr (MODE <= 1) {
-    loss_gemm_kernel<BF, MODE, 128, 256, 1, 4, 32, 3><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
+    loss_gemm_kernel<BF, MODE, 128, 256, 1, 4, 3><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
   } else {
     const int nl = (MODE == 2 ? a.vn : a.Mp) / LK_BL, nr = (a.H + 191) / 192;
-    loss_gemm_kernel<BF, MODE, LK_BL, 192, 2, 2, 32, 4><<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
+    loss_gemm_kernel<BF, MODE, LK_BL, 192, 2, 2, 4><<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
   }
 }
 
 template <bool BF>
 void lk_forward(LossArgs a, const LossPlan& p, hipStream_t st) {
   loss_rows_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
-  loss_gather_kernel<<<dim3((unsigned)(((long)p.Mp * (p.Hp / 8) + 255) / 256)), dim3(256), 0, st>>>(a);
+  loss_layout_kernel<<<dim3((unsigned)(((long)(p.Mp + a.Vp) * (p.Hp / 8) + 255) / 256)), dim3(256), 0, st>>>(a);
   a.v0 = 0;
   a.vn = p.vtiles * (p.small ? 64 : 256);
   lk_gemm<BF, 0>(a, p, st);
-  loss_join_kernel<BF><<<dim3(p.Mp / 64), dim3(256), 0, st>>>(a, p.vtiles);
+  loss_join_kernel<BF><<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
   if (a.mode != 2) loss_sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
 }
 
@@ -719,35 +681,36 @@ void lk_state(LossArgs& a, const LossPlan& p, void* state) {
   a.lse = (float*)(a.lab + p.Mp);
   a.rl = a.lse + p.Mp;
   a.pos = (int*)(a.rl + p.Mp);
-  a.Mp = p.Mp, a.Hp = p.Hp;
+  a.Mp = p.Mp, a.Hp = p.Hp, a.Vp = p.vtiles * (p.small ? 64 : 256);
 }
 
 }  // namespace
 
 extern "C" {
 
-// out[0..5]: rows and columns of hc; 32-bit words of state, of the forward's and of the
-// backward's workspace (in units of 64 words); elements of d are part of the last
+// out[0..5]: rows and columns of hc, rows of ec (as many columns); state and the forward's and
+// the backward's workspace, in units of 256 bytes
 int sg_loss_plan(int N, int V, int H, void* out) {
   if (lk_bad(N, V, H, 0)) return 1;
   const LossPlan p = lk_plan(N, V, H);
   int* o = (int*)out;
   o[0] = p.Mp;
   o[1] = p.Hp;
-  o[2] = (64 + 4 * p.Mp + N + 63) / 64;
-  o[3] = (int)((2L * p.vtiles * p.Mp + 63) / 64);
-  o[4] = (int)((64 + p.Mp + (long)p.Mp * p.piece / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
+  o[2] = p.vtiles * (p.small ? 64 : 256);
+  o[3] = (64 + 4 * p.Mp + N + 63) / 64;
+  o[4] = (int)((2L * p.vtiles * p.Mp + 63) / 64);
+  o[5] = (int)((64 + p.Mp + (long)p.Mp * p.piece / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
   return 0;
 }
 
 // mode: 0 mean, 1 sum (loss [1]), 2 none (loss [N])
-int sg_loss_fwd(const void* h, const void* table, const void* labels, int is64, int ignore, void* hc, void* state,
-                void* ws, void* loss, int N, int V, int H, int mode, int fp16, hipStream_t st) {
+int sg_loss_fwd(const void* h, const void* table, const void* labels, int is64, int ignore, void* hc, void* ec,
+                void* state, void* ws, void* loss, int N, int V, int H, int mode, int fp16, hipStream_t st) {
   if (lk_bad(N, V, H, mode)) return 1;
   const LossPlan p = lk_plan(N, V, H);
   LossArgs a = {};
   a.h = (const uint16_t*)h, a.table = (const uint16_t*)table, a.labels = labels, a.is64 = is64, a.ignore = ignore;
-  a.hc = (uint16_t*)hc, a.loss = (float*)loss, a.part = (float2*)ws;
+  a.hc = (uint16_t*)hc, a.ec = (uint16_t*)ec, a.loss = (float*)loss, a.part = (float2*)ws;
   a.N = N, a.V = V, a.H = H, a.mode = mode;
   lk_state(a, p, state);
   fp16 ? lk_forward<false>(a, p, st) : lk_forward<true>(a, p, st);
@@ -755,12 +718,12 @@ int sg_loss_fwd(const void* h, const void* table, const void* labels, int is64, 
 }
 
 // g: the gradient of loss ([1], none: [N]); dh or dtable may be null (not wanted)
-int sg_loss_bwd(const void* hc, const void* table, void* state, const void* g, void* ws, void* dh, void* dtable, int N,
+int sg_loss_bwd(const void* hc, const void* ec, void* state, const void* g, void* ws, void* dh, void* dtable, int N,
                 int V, int H, int mode, int fp16, hipStream_t st) {
   if (lk_bad(N, V, H, mode)) return 1;
   const LossPlan p = lk_plan(N, V, H);
   LossArgs a = {};
-  a.hc = (uint16_t*)const_cast<void*>(hc), a.table = (const uint16_t*)table, a.g = (const float*)g;
+  a.hc = (uint16_t*)const_cast<void*>(hc), a.ec = (uint16_t*)const_cast<void*>(ec), a.g = (const float*)g;
   a.dh = (uint16_t*)dh, a.dtable = (uint16_t*)dtable;
   a.N = N, a.V = V, a.H = H, a.mode = mode;
   lk_state(a, p, state);
