@@ -10,13 +10,12 @@
 // block reads the count from the device and ends at once behind it (an SMS batch labels
 // about a third of its positions).
 //
-//   forward   loss_gemm<0>: a tile's logits stay in the accumulators; each row's maximum
+//   forward   loss_logits<0>: a tile's logits stay in the accumulators; each row's maximum
 //             and sum of exponentials over the tile go out (8 bytes a row and tile);
 //             loss_join: L and loss, with z_i[y_i] as a dot product of its own
-//   backward  per piece of the vocabulary: loss_gemm<1> recomputes the tile's logits and
-//             writes d in the inputs' type; loss_gemm<2>: the piece's rows of dE;
-//             loss_gemm<3>: dh's share, fp32, the piece's columns split over blocks;
-//             loss_dh sums the shares in order and puts the rows back (ignored: zeros)
+//   backward  per piece of the vocabulary: loss_logits<1> recomputes the tile's logits and
+//             writes d in the inputs' type; loss_grad: the piece's rows of dE, and dh's
+//             share, fp32, the piece's columns split over blocks; loss_dh sums the shares in order and puts the rows back (ignored: zeros)
 //
 // Four products of 2 n V H flops where keeping the logits would need three: z is needed in
 // fp32 (its rounding to 16 bits would put errors of per cents into exp), and storing it
@@ -64,6 +63,7 @@ struct LossArgs {
   int v0, vn;                       // piece: first row, rows (of them < V - v0 real)
   int splits, want, most, first;    // dh: shares of Mp rows in the workspace; blocks wanted; splits at most
   int bl, nr;                       // dh: rows of a tile, tiles over H
+  int t2;                           // blocks of dE, a multiple of 8
 };
 
 template <bool BF>
@@ -259,12 +259,17 @@ __device__ __forceinline__ int lk_splits(int rows, int tiles, const LossArgs& a)
 // MODE 3: lane = hidden rows, register = H, k = a split of the piece.
 // 32 k-values a step, ST buffers: the copies of the next ST - 1 steps are in flight.
 template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST>
-__global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
-  constexpr int NW = WL * WR, TL = BL / WL, TR = BR / WR, FL = TL / 32, FR = TR / 32;
-  constexpr bool LCOL = MODE == 2, RCOL = MODE >= 2;
-  constexpr int BK = LK_PANEL, STAGE = (BL + BR) * BK, NI = (BL + BR) / 16 / NW;
+struct LkTile {
+  static constexpr int NW = WL * WR, TL = BL / WL, TR = BR / WR, FL = TL / 32, FR = TR / 32;
+  static constexpr int BK = LK_PANEL, STAGE = (BL + BR) * BK, NI = (BL + BR) / 16 / NW;
   static_assert(ST * STAGE * 2 <= 160 * 1024 && BL % (32 * WL) == 0 && BR % (32 * WR) == 0, "tile");
-  __shared__ __attribute__((aligned(16))) uint16_t sm[ST * STAGE];
+  static __device__ __forceinline__ void run(const LossArgs& a, int block, uint16_t* sm);
+};
+
+template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST>
+__device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const LossArgs& a, int block,
+                                                                          uint16_t* sm) {
+  constexpr bool LCOL = MODE == 2, RCOL = MODE >= 2;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int wl = wave / WR, wr = wave % WR;
   const int cnt = a.cnt[0];
@@ -276,7 +281,7 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   // tiles only (the grid holds all rows'): else a few XCDs would have all the work
   int t, z = 0;
   {
-    const int T = nl * nr * splits, x = blockIdx.x & 7, q = T >> 3, r = T & 7, i = blockIdx.x >> 3;
+    const int T = nl * nr * splits, x = block & 7, q = T >> 3, r = T & 7, i = block >> 3;
     if (i >= q + (x < r)) return;
     t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
   }
@@ -455,6 +460,27 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_gemm_kernel(LossArgs a) {
   }
 }
 
+template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST>
+__global__ void __launch_bounds__(WL * WR * 64) loss_logits_kernel(LossArgs a) {
+  typedef LkTile<BF, MODE, BL, BR, WL, WR, ST> Tile;
+  __shared__ __attribute__((aligned(16))) uint16_t sm[ST * Tile::STAGE];
+  Tile::run(a, blockIdx.x, sm);
+}
+
+// dE's tiles (the first a.t2 blocks), then dh's: one launch, because neither fills the card
+// by itself (16384 ids and 576 columns: 384 tiles for 512 places) and dh's, split as finely
+// as one likes, fill the places that dE's leave.
+template <bool BF, int BL, int BR, int WL, int WR, int ST>
+__global__ void __launch_bounds__(WL * WR * 64) loss_grad_kernel(LossArgs a) {
+  typedef LkTile<BF, 2, BL, BR, WL, WR, ST> Table;
+  typedef LkTile<BF, 3, BL, BR, WL, WR, ST> Hidden;
+  __shared__ __attribute__((aligned(16))) uint16_t sm[ST * Table::STAGE];
+  if ((int)blockIdx.x < a.t2)
+    Table::run(a, blockIdx.x, sm);
+  else
+    Hidden::run(a, blockIdx.x - a.t2, sm);
+}
+
 // ---- joins -----------------------------------------------------------------------------
 // 16 rows a block: L from the tiles' (maximum, sum), the label's logit, the loss.
 template <bool BF>
@@ -610,32 +636,37 @@ LossPlan lk_plan(int N, int V, int H) {
   // dh: blocks over the card, each with at least 4 steps of k
   const int bl = p.small ? 64 : LK_BL, br = p.small ? 64 : 192;
   const int tiles = p.Mp / bl * ((H + br - 1) / br);
-  p.want = 512;
+  p.want = 768;
   p.most = p.piece / (4 * LK_K) < 64 ? p.piece / (4 * LK_K) : 64;
   const int s = (p.want + tiles - 1) / tiles;
   p.splits = s < p.most ? s : p.most;
   return p;
 }
 
-// dh: as many blocks as any count of rows may want (lk_splits: tiles x splits is at most
-// tiles + want, and at most the workspace's shares)
-unsigned lk_grid(int mode, int nl, int nr, const LossArgs& a) {
-  if (mode != 3) return (unsigned)(nl * nr);
-  const long all = (long)nl * nr * a.splits, some = (long)nl * nr + a.want;
-  return (unsigned)(((all < some ? all : some) + 7) / 8 * 8);
+template <bool BF, int MODE>
+void lk_logits(const LossArgs& a, const LossPlan& p, hipStream_t st) {
+  if (p.small)
+    loss_logits_kernel<BF, MODE, 64, 64, 2, 2, 4><<<dim3(a.Mp / 64 * (a.vn / 64)), dim3(256), 0, st>>>(a);
+  else
+    loss_logits_kernel<BF, MODE, 128, 256, 1, 4, 3><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
 }
 
-template <bool BF, int MODE>
-void lk_gemm(const LossArgs& a, const LossPlan& p, hipStream_t st) {
-  if (p.small) {
-    const int nl = (MODE == 2 ? a.vn : a.Mp) / 64, nr = MODE >= 2 ? (a.H + 63) / 64 : a.vn / 64;
-    loss_gemm_kernel<BF, MODE, 64, 64, 2, 2, 4><<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
-  } else if constexpr (MODE <= 1) {
-    loss_gemm_kernel<BF, MODE, 128, 256, 1, 4, 3><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
-  } else {
-    const int nl = (MODE == 2 ? a.vn : a.Mp) / LK_BL, nr = (a.H + 191) / 192;
-    loss_gemm_kernel<BF, MODE, LK_BL, 192, 2, 2, 4><<<dim3(lk_grid(MODE, nl, nr, a)), dim3(256), 0, st>>>(a);
+// dh has as many blocks as any count of rows may want (lk_splits: tiles x splits is at most
+// tiles + want, and at most the workspace's shares).
+template <bool BF>
+void lk_grads(LossArgs a, const LossPlan& p, hipStream_t st) {
+  a.t2 = a.dtable != nullptr ? (a.vn / a.bl * a.nr + 7) / 8 * 8 : 0;
+  long t3 = 0;
+  if (a.dh != nullptr) {
+    const long nl = a.Mp / a.bl, all = nl * a.nr * a.splits, some = nl * a.nr + a.want;
+    t3 = all < some ? all : some;
   }
+  if (a.t2 + t3 == 0) return;
+  const dim3 grid((unsigned)(a.t2 + t3));
+  if (p.small)
+    loss_grad_kernel<BF, 64, 64, 2, 2, 4><<<grid, dim3(256), 0, st>>>(a);
+  else
+    loss_grad_kernel<BF, LK_BL, 192, 2, 2, 4><<<grid, dim3(256), 0, st>>>(a);
 }
 
 template <bool BF>
@@ -644,7 +675,7 @@ void lk_forward(LossArgs a, const LossPlan& p, hipStream_t st) {
   loss_layout_kernel<<<dim3((unsigned)(((long)(p.Mp + a.Vp) * (p.Hp / 8) + 255) / 256)), dim3(256), 0, st>>>(a);
   a.v0 = 0;
   a.vn = p.vtiles * (p.small ? 64 : 256);
-  lk_gemm<BF, 0>(a, p, st);
+  lk_logits<BF, 0>(a, p, st);
   loss_join_kernel<BF><<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
   if (a.mode != 2) loss_sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
 }
@@ -659,9 +690,8 @@ void lk_backward(LossArgs a, const LossPlan& p, hipStream_t st) {
     a.v0 = v0;
     a.vn = vp - v0 < p.piece ? vp - v0 : p.piece;
     a.first = v0 == 0;
-    lk_gemm<BF, 1>(a, p, st);
-    if (a.dtable != nullptr) lk_gemm<BF, 2>(a, p, st);
-    if (a.dh != nullptr) lk_gemm<BF, 3>(a, p, st);
+    lk_logits<BF, 1>(a, p, st);
+    lk_grads<BF>(a, p, st);
   }
   if (a.dh != nullptr)
     loss_dh_kernel<BF><<<dim3((unsigned)(((long)a.N * (a.H / 4) + 255) / 256)), dim3(256), 0, st>>>(a);
