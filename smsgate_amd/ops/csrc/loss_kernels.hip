@@ -461,7 +461,7 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
 }
 
 template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST>
-__global__ void __launch_bounds__(WL * WR * 64) loss_logits_kernel(LossArgs a) {
+__global__ void __launch_bounds__(WL * WR * 64, 3) loss_logits_kernel(LossArgs a) {
   typedef LkTile<BF, MODE, BL, BR, WL, WR, ST> Tile;
   __shared__ __attribute__((aligned(16))) uint16_t sm[ST * Tile::STAGE];
   Tile::run(a, blockIdx.x, sm);
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(WL * WR * 64) loss_logits_kernel(LossArgs a) {
 // by itself (16384 ids and 576 columns: 384 tiles for 512 places) and dh's, split as finely
 // as one likes, fill the places that dE's leave.
 template <bool BF, int BL, int BR, int WL, int WR, int ST>
-__global__ void __launch_bounds__(WL * WR * 64) loss_grad_kernel(LossArgs a) {
+__global__ void __launch_bounds__(WL * WR * 64, 3) loss_grad_kernel(LossArgs a) {
   typedef LkTile<BF, 2, BL, BR, WL, WR, ST> Table;
   typedef LkTile<BF, 3, BL, BR, WL, WR, ST> Hidden;
   __shared__ __attribute__((aligned(16))) uint16_t sm[ST * Table::STAGE];
@@ -648,7 +648,7 @@ void lk_logits(const LossArgs& a, const LossPlan& p, hipStream_t st) {
   if (p.small)
     loss_logits_kernel<BF, MODE, 64, 64, 2, 2, 4><<<dim3(a.Mp / 64 * (a.vn / 64)), dim3(256), 0, st>>>(a);
   else
-    loss_logits_kernel<BF, MODE, 128, 256, 1, 4, 3><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
+    loss_logits_kernel<BF, MODE, 128, 256, 1, 4, 2><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
 }
 
 // dh has as many blocks as any count of rows may want (lk_splits: tiles x splits is at most
@@ -666,7 +666,7 @@ void lk_grads(LossArgs a, const LossPlan& p, hipStream_t st) {
   if (p.small)
     loss_grad_kernel<BF, 64, 64, 2, 2, 4><<<grid, dim3(256), 0, st>>>(a);
   else
-    loss_grad_kernel<BF, LK_BL, 192, 2, 2, 4><<<grid, dim3(256), 0, st>>>(a);
+    loss_grad_kernel<BF, LK_BL, 192, 4, 1, 2><<<grid, dim3(256), 0, st>>>(a);
 }
 
 template <bool BF>
