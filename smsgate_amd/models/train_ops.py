@@ -229,6 +229,11 @@ def _vec16(H: int, *tensors: torch.Tensor) -> int:
     return int((ptrs | H * tensors[0].element_size()) % 16 == 0)
 
 
+@functools.lru_cache(maxsize=256)
+def _embed_units(entries: int, V: int, H: int) -> int:
+    return _lib().sg_embed_grad_ws(entries, V, H)
+
+
 class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table: torch.Tensor, ids: torch.Tensor, add: Optional[torch.Tensor], scale: float):
@@ -244,8 +249,7 @@ class _Embed(torch.autograd.Function):
         ctx.save_for_backward(ids, add)
         # all that the gradient's launch needs but the pointers: autograd's thread pays
         # more for each Python step than the caller's
-        ctx.plan = (lib.sg_embed_grad, dev, n, V, H, scale, code, is64,
-                    lib.sg_embed_grad_ws(n if add is None else 2 * n, V, H))
+        ctx.plan = (lib.sg_embed_grad, dev, n, V, H, scale, code, is64, _embed_units(n if add is None else 2 * n, V, H))
         return x
 
     @staticmethod
@@ -279,8 +283,8 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch
         raise TypeError("embed_lookup: ids must be int32 or int64")
     if add_ids is not None and (add_ids.shape != ids.shape or add_ids.dtype != ids.dtype):
         raise ValueError("embed_lookup: add_ids must have the shape and type of ids")
-    if min(table.shape) < 1 or table.shape[0] >= 1 << 30 or ids.numel() >= 1 << 30:
-        raise ValueError("embed_lookup: 1 <= V < 2^30, H >= 1, fewer than 2^30 ids")
+    if not (1 <= table.shape[0] < 1 << 30 and 1 <= table.shape[1] <= 1 << 20) or ids.numel() >= 1 << 29:
+        raise ValueError("embed_lookup: 1 <= V < 2^30, 1 <= H <= 2^20, fewer than 2^29 ids")
     _on_gpu("embed_lookup", table, ids, add_ids)
     return _Embed.apply(table, ids, add_ids, float(scale))
 
@@ -289,11 +293,26 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -
     return _Attention.apply(q, k, v, scale)
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and on a 16-byte border (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """``t`` [B, heads, T, D] itself when its rows can be read 16 bytes at a time, else a copy."""
-    if t.stride(3) == 1 and (t.stride(0) | t.stride(1) | t.stride(2)) % 8 == 0 and t.data_ptr() % 16 == 0:
+    b, h, r, c = t.stride()
+    if c == 1 and (b | h | r) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
-    return t.contiguous()
+    return t.contiguous() if c != 1 or (b | h | r) % 8 else t.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_plan(B: int, T: int, nh: int, nkv: int, D: int, fp16: int):
+    """32-bit words of the row statistics and of the backward's workspace."""
+    lib = _lib()
+    stats = B * nh * lib.sg_attn_rows(T)
+    return stats, stats + 256 * fp16 + (2 * B * nh * T * D if lib.sg_attn_split(B, T, nh, nkv) else 0)
 
 
 class _TiledAttention(torch.autograd.Function):
@@ -302,34 +321,37 @@ class _TiledAttention(torch.autograd.Function):
         B, nh, T, D = q.shape
         nkv, dev, fp16 = k.shape[1], q.get_device(), int(q.dtype == torch.float16)
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        lengths = None if lengths is None else lengths.contiguous()
+        if lengths is not None:
+            lengths = lengths.contiguous()
         lib = _lib()
-        rows = lib.sg_attn_rows(T)
+        stats, words = _attn_plan(B, T, nh, nkv, D, fp16)
         out = torch.empty(B, T, nh * D, dtype=q.dtype, device=q.device)
-        # what rounding took from out, for the backward's D (none: no gradient will be asked)
-        olo = torch.empty_like(out) if any(ctx.needs_input_grad[:3]) else None
-        lse = torch.empty(B, nh, rows, dtype=torch.float32, device=q.device)
+        # the rows' statistics, and behind them what rounding took from out, for the
+        # backward's D (not where no gradient will be asked for)
+        grad = any(ctx.needs_input_grad[:3])
+        keep = torch.empty(stats + (B * T * nh * D // 2 if grad else 0), dtype=torch.float32, device=q.device)
+        lse = keep.data_ptr()
+        olo = lse + 4 * stats if grad else None
         strides = (ctypes.c_long * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
         dims = (B, T, nh, nkv, D, int(causal), fp16, scale)
         _run(dev, "attn_fwd", lib.sg_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), ops._p(lengths),
-             out.data_ptr(), ops._p(olo), lse.data_ptr(), strides, *dims)
-        ctx.save_for_backward(q, k, v, lengths, out, olo, lse)
-        words = B * nh * rows + 256 * fp16 + (2 * B * nh * T * D if lib.sg_attn_split(B, T, nh, nkv) else 0)
-        ctx.plan = (lib.sg_attn_bwd, dev, strides, dims, words)
+             out.data_ptr(), olo, lse, strides, *dims)
+        ctx.save_for_backward(q, k, v, lengths, out, keep)
+        ctx.plan = (lib.sg_attn_bwd, dev, strides, dims, stats, words)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: torch.Tensor):
-        q, k, v, lengths, out, olo, lse = ctx.saved_tensors
-        fn, dev, strides, dims, words = ctx.plan
-        dout = dout.contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
+        q, k, v, lengths, out, keep = ctx.saved_tensors
+        fn, dev, strides, dims, stats, words = ctx.plan
+        dout = _aligned(dout)
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        ws = lse.new_empty(words)
+        ws = keep.new_empty(words)
+        lse = keep.data_ptr()
         _run(dev, "attn_bwd", fn, q.data_ptr(), k.data_ptr(), v.data_ptr(), ops._p(lengths), out.data_ptr(),
-             olo.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), strides, *dims)
+             lse + 4 * stats, lse, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), strides,
+             *dims)
         return dq, dk, dv, None, None, None
 
 
@@ -367,44 +389,49 @@ def tiled_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and on a 16-byte border (a copy where it is not)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+@functools.lru_cache(maxsize=256)
+def _loss_plan(N: int, V: int, H: int):
+    """Elements of hc, ec and state (in the inputs' 16 bits), 32-bit words of the forward's and
+    the backward's workspace."""
+    plan = (ctypes.c_int * 6)()
+    _ok(_lib().sg_loss_plan(N, V, H, plan), "loss_plan")
+    rows, cols, vrows, state, fwd, bwd = plan
+    return rows * cols, vrows * cols, state * 128, fwd * 64, bwd * 64
 
 
 class _LmLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, table, labels, mode: int, ignore: int):
         V, H = table.shape
-        N, dev, fp16, is64 = labels.numel(), h.get_device(), int(h.dtype == torch.float16), int(
-            labels.dtype == torch.int64)
+        N, dev, fp16 = labels.numel(), h.get_device(), int(h.dtype == torch.float16)
         shape, h, table, labels = h.shape, _aligned(h), _aligned(table), labels.contiguous()
         lib = _lib()
-        plan = (ctypes.c_int * 6)()
-        _ok(lib.sg_loss_plan(N, V, H, plan), "loss_plan")
-        # the labelled rows and the table as the products read them, kept for the backward
-        hc, ec = h.new_empty(plan[0], plan[1]), h.new_empty(plan[2], plan[1])
-        state = torch.empty(plan[3] * 64, dtype=torch.int32, device=h.device)
-        ws = torch.empty(plan[4] * 64, dtype=torch.float32, device=h.device)
+        nhc, nec, nst, fwd, bwd = _loss_plan(N, V, H)
+        # the labelled rows and the table as the products read them, and the rows' places and
+        # statistics: kept for the backward
+        keep = h.new_empty(nhc + nec + nst)
+        ws = torch.empty(fwd, dtype=torch.float32, device=h.device)
         loss = torch.empty(labels.shape if mode == 2 else (), dtype=torch.float32, device=h.device)
-        _run(dev, "loss_fwd", lib.sg_loss_fwd, h.data_ptr(), table.data_ptr(), labels.data_ptr(), is64, ignore,
-             hc.data_ptr(), ec.data_ptr(), state.data_ptr(), ws.data_ptr(), loss.data_ptr(), N, V, H, mode, fp16)
-        ctx.save_for_backward(hc, ec, state)
-        ctx.plan = (lib.sg_loss_bwd, dev, shape, (N, V, H, mode, fp16), plan[5] * 64)
+        hc = keep.data_ptr()
+        ec, state = hc + 2 * nhc, hc + 2 * (nhc + nec)
+        _run(dev, "loss_fwd", lib.sg_loss_fwd, h.data_ptr(), table.data_ptr(), labels.data_ptr(),
+             int(labels.dtype == torch.int64), ignore, hc, ec, state, ws.data_ptr(), loss.data_ptr(), N, V, H, mode, fp16)
+        ctx.save_for_backward(keep)
+        ctx.plan = (lib.sg_loss_bwd, dev, shape, (N, V, H, mode, fp16), nhc, nec, bwd)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        hc, ec, state = ctx.saved_tensors
-        fn, dev, shape, dims, words = ctx.plan
+        (keep,) = ctx.saved_tensors
+        fn, dev, shape, dims, nhc, nec, words = ctx.plan
         g = g.contiguous()
-        dh = hc.new_empty(shape) if ctx.needs_input_grad[0] else None
-        dt = hc.new_empty(dims[1], dims[2]) if ctx.needs_input_grad[1] else None
+        hc = keep.data_ptr()
+        dh = keep.new_empty(shape) if ctx.needs_input_grad[0] else None
+        dt = keep.new_empty(dims[1], dims[2]) if ctx.needs_input_grad[1] else None
         ws = g.new_empty(words)
-        _run(dev, "loss_bwd", fn, hc.data_ptr(), ec.data_ptr(), state.data_ptr(), g.data_ptr(), ws.data_ptr(),
-             ops._p(dh), ops._p(dt), *dims)
+        _run(dev, "loss_bwd", fn, hc, hc + 2 * nhc, hc + 2 * (nhc + nec), g.data_ptr(), ws.data_ptr(), ops._p(dh),
+             ops._p(dt), *dims)
         return dh, dt, None, None, None
 
 

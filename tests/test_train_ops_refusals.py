@@ -18,6 +18,7 @@ def _ids(*shape, dtype=torch.long):
     (_ids(3), torch.zeros(4, 8), _ids(4), ValueError),                              # add_ids of another shape
     (_ids(3), torch.zeros(4, 8), _ids(3, dtype=torch.int32), ValueError),           # or type
     (_ids(3), torch.zeros(0, 8), None, ValueError),                                 # an empty table
+    (_ids(3), torch.empty(1, 1 << 21, device="meta"), None, ValueError),             # rows too wide
     (_ids(3), torch.zeros(4, 8), None, ValueError),                                 # not on a GPU
 ])
 def test_embed_lookup_refuses(ids, table, add, err):
