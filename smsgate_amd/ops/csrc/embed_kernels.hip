@@ -10,22 +10,26 @@
 //
 // Both directions are bound by memory: the rows read, x / dx, and dE written once whole.
 //   * up to EG_SMALL entries (one message): ONE launch; every block scans all the ids for
-//     its 16 rows of dE.  A launch costs more than the work.
+//     its 16 rows of dE.  A launch costs more than the work (45 positions of 256 over 8192
+//     ids, fp32: 2.5 us forward, 4.8 us gradient, of which 8.4 MB of dE take 2).
 //   * else the entries are sorted by id (stable, so each id's positions stay in order), in
 //     one launch up to EG_RANGE entries, else in three launches a pass of 8 bits; then one
 //     wave a row of dE sums its positions (rows of no entry are zeroed there, so dE is
 //     written once).  An id of many entries (a separator, the shared prompt) would leave
 //     one wave with thousands of rows: runs of EG_CHUNK sorted entries of one id are summed
 //     beforehand, and rows of over EG_COOP terms are shared by the block's 4 waves.
+// Measured: 7808 positions with second rows, 576 fp32 over 8576 ids: 7 us forward (2.6 TB/s
+// with the rows from L2), 18 sort, 5 chunks, 14 rows.  130999 positions, 960 bf16 over 49152
+// ids: 75 us forward (4.6 TB/s, a large copy's 4.8), 41 sort, 42 chunks, 72 rows.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 namespace {
 
 constexpr int EG_SMALL = 256;    // entries that the one-launch gradient takes
-// Entries, and ids, that the one-launch sort takes: its blocks each read every id, so its time
-// grows by 1.4 us a thousand entries (25 us at 15616, 192 at 130999), the passes' by 0.1
-// from 30 us (40 at 130999).
+// Entries, and ids, that the one-launch sort takes.  Its blocks each read every id: 18 us at
+// 15616 entries, where the passes need seven launches (about 30 us); a form of it that reads
+// more than the registers hold took 192 us at 130999, the passes 41.
 constexpr int EG_RANGE = 1 << 14;
 constexpr int EG_RANGE_V = 1 << 18;
 constexpr int EG_CHUNK = 32;     // sorted entries of one id summed beforehand
@@ -141,14 +145,14 @@ __device__ __forceinline__ unsigned long long eg_peers(uint32_t digit, bool on) 
   return m;
 }
 
-// One stable counting pass of a wave's entries, 64 at a time: `cnt` (this wave's 256
-// counters) holds each digit's next place; PLACE false only counts.
-template <bool PLACE, typename F>
+// One stable step of a wave's entries, 64 at a time: `cnt` (this wave's 256 counters) holds
+// each digit's next place.  (Counting alone needs no order: LDS additions of whole numbers.)
+template <typename F>
 __device__ __forceinline__ void eg_wave_step(volatile int* cnt, uint32_t digit, bool on, int lane, F place) {
   const unsigned long long peers = eg_peers(digit, on);
   const int rank = __popcll(peers & ((1ull << lane) - 1));
   if (on) {
-    if (PLACE) place(cnt[digit] + rank);
+    place(cnt[digit] + rank);
     __builtin_amdgcn_wave_barrier();
     if (rank == 0) cnt[digit] = cnt[digit] + __popcll(peers);
     __builtin_amdgcn_wave_barrier();
@@ -156,9 +160,9 @@ __device__ __forceinline__ void eg_wave_step(volatile int* cnt, uint32_t digit, 
 }
 
 // Sorts up to EG_RANGE entries in one launch: block b places the entries of the 256 ids
-// [256 b, 256 b + 256) by itself.  It reads every id twice (from L2: 8 n2 bytes a block), to
-// count its ids and the entries of lower ids, which is where its own begin, and to place
-// them; a wave owns a run of entries, so places keep their order.  Writes seg of its ids.
+// [256 b, 256 b + 256) by itself.  It reads every id (from L2: 8 n2 bytes a block), counts its
+// own and the entries of lower ids, which is where its own begin, and places them; a wave
+// owns a run of entries, so places keep their order.  Writes seg of its ids.
 __global__ void __launch_bounds__(1024) embed_range_sort_kernel(const void* __restrict__ ids,
                                                                 const void* __restrict__ add, int is64, int n, int n2,
                                                                 int V, uint32_t* __restrict__ keys,
@@ -172,23 +176,22 @@ __global__ void __launch_bounds__(1024) embed_range_sort_kernel(const void* __re
   volatile int* mine = cnt + wave * 256;
   for (int i = tid; i < 16 * 256; i += 1024) cnt[i] = 0;
   __syncthreads();
-  // f(entry, key, in range) for the wave's entries, 8 loads in flight
+  // the wave's entries stay in registers: f(entry, key, in range)
+  constexpr int R = EG_RANGE / 16 / 64;
+  uint32_t key[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int e = w0 + 64 * r + lane;
+    key[r] = e < w1 ? eg_key(ids, add, is64, n, e, V) : (uint32_t)V;
+  }
   auto walk = [&](auto f) {
-    for (int e0 = w0; e0 < w1; e0 += 512) {
-      uint32_t k[8];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const int e = e0 + 64 * r + lane;
-        k[r] = e < w1 ? eg_key(ids, add, is64, n, e, V) : (uint32_t)V;
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) f(e0 + 64 * r + lane, k[r], k[r] - v0 < 256u && k[r] < (uint32_t)V);
-    }
+    for (int r = 0; r < R; ++r) f(w0 + 64 * r + lane, key[r], key[r] - v0 < 256u && key[r] < (uint32_t)V);
   };
   int below = 0;
   walk([&](int, uint32_t k, bool on) {
     below += k < v0;  // (an id of no row is V: in no range and below none)
-    if (__any(on)) eg_wave_step<false>(mine, (k - v0) & 255u, on, lane, [](int) {});
+    if (on) atomicAdd(&cnt[wave * 256 + (k - v0)], 1);
   });
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o, 64);
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(1024) embed_range_sort_kernel(const void* __re
   __syncthreads();
   walk([&](int e, uint32_t k, bool on) {
     if (__any(on))
-      eg_wave_step<true>(mine, (k - v0) & 255u, on, lane, [&](int at) {
+      eg_wave_step(mine, (k - v0) & 255u, on, lane, [&](int at) {
         keys[at] = k;
         ents[at] = e;
       });
@@ -300,7 +303,7 @@ __global__ void __launch_bounds__(256) embed_scatter_kernel(const uint32_t* __re
   for (int r = 0; r < EG_TILE / 256; ++r) {
     const int e = w0 + 64 * r + lane;
     key[r] = e < w1 ? eg_load(keys, ids, add, is64, n, e, V) : 0u;
-    eg_wave_step<false>(mine, (key[r] >> sh) & 255u, e < w1, lane, [](int) {});
+    if (e < w1) atomicAdd(&cnt[wave * 256 + ((key[r] >> sh) & 255u)], 1);
   }
   if (wave == 0) {  // exclusive sums of the digits' totals, 4 a lane
     const int* total = hist + (size_t)256 * gridDim.x + 4 * lane;
@@ -333,7 +336,7 @@ __global__ void __launch_bounds__(256) embed_scatter_kernel(const uint32_t* __re
   for (int r = 0; r < EG_TILE / 256; ++r) {
     const int e = w0 + 64 * r + lane;
     const int ent = keys != nullptr && e < w1 ? ents[e] : e;
-    eg_wave_step<true>(mine, (key[r] >> sh) & 255u, e < w1, lane, [&](int at) {
+    eg_wave_step(mine, (key[r] >> sh) & 255u, e < w1, lane, [&](int at) {
       keys_out[at] = key[r];
       ents_out[at] = ent;
     });
@@ -351,20 +354,20 @@ __global__ void __launch_bounds__(256) embed_bounds_kernel(const uint32_t* __res
 }
 
 // ---- sums ----------------------------------------------------------------------------
-// acc += the dx rows of sorted entries [e0, e1), in order, 8 rows in flight.
-template <typename T, int VEC>
+// acc += the dx rows of sorted entries [e0, e1), in order, FLY rows in flight.
+template <typename T, int VEC, int FLY = 8>
 __device__ __forceinline__ void eg_sum_entries(float (&acc)[VEC], const int* __restrict__ ents,
                                                const T* __restrict__ dx, int n, int H, int c, int e0, int e1) {
   typedef EgVec<T, VEC> vec;
-  for (int e = e0; e < e1; e += 8) {
-    vec d[8];
+  for (int e = e0; e < e1; e += FLY) {
+    vec d[FLY];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < FLY; ++k) {
       const int en = ents[min(e + k, e1 - 1)], row = en < n ? en : en - n;
       d[k] = reinterpret_cast<const vec*>(dx + (size_t)row * H)[c];
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < FLY; ++k)
       if (e + k < e1) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[j] += eg_f(d[k].v[j]);
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(256) embed_chunk_kernel(const uint32_t* __rest
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-  eg_sum_entries<T, VEC>(acc, ents, dx, n, H, c, e0, e0 + EG_CHUNK);
+  eg_sum_entries<T, VEC, EG_CHUNK>(acc, ents, dx, n, H, c, e0, e0 + EG_CHUNK);
 #pragma unroll
   for (int j = 0; j < VEC; ++j) part[(size_t)ch * H + (size_t)c * VEC + j] = acc[j];
 }

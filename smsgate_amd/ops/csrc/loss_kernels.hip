@@ -5,17 +5,17 @@
 //   d_i[v] = w_i (exp(z_i[v] - L_i) - [v = y_i]),  dh = f d E,  dE = f d^T h
 //
 // h [N, H] and E [V, H] in bf16 or fp16, H a multiple of 8, any N and V.  Rows whose label
-// is ignore_index are left out before any product: loss_rows lists the others, loss_gather
-// copies them together ([Mp][Hp], zero behind the last row and column), and every later
-// block reads the count from the device and ends at once behind it (an SMS batch labels
-// about a third of its positions).
+// is ignore_index are left out before any product: loss_rows lists the others, loss_layout
+// copies them together, and every later block reads the count from the device and ends at
+// once behind it (an SMS batch labels about a third of its positions).
 //
 //   forward   loss_logits<0>: a tile's logits stay in the accumulators; each row's maximum
 //             and sum of exponentials over the tile go out (8 bytes a row and tile);
 //             loss_join: L and loss, with z_i[y_i] as a dot product of its own
 //   backward  per piece of the vocabulary: loss_logits<1> recomputes the tile's logits and
 //             writes d in the inputs' type; loss_grad: the piece's rows of dE, and dh's
-//             share, fp32, the piece's columns split over blocks; loss_dh sums the shares in order and puts the rows back (ignored: zeros)
+//             shares, fp32, the piece's columns split over blocks; loss_dh sums the shares in
+//             order and puts the rows back (ignored: zeros)
 //
 // Four products of 2 n V H flops where keeping the logits would need three: z is needed in
 // fp32 (its rounding to 16 bits would put errors of per cents into exp), and storing it
@@ -26,11 +26,17 @@
 //
 // Products: v_mfma_f32_32x32x16, result in lane l: column l & 31 (the "lane" side: a hidden
 // row, or a vocabulary row for dE), rows (r & 3) + 8 (r >> 2) + 4 (l >> 5) (the "register"
-// side).  Operands whose k runs along memory are read from LDS as rows, others by
-// transposing reads (ds_read_b64_tr_b16) of tiles kept as they lie in memory, so no
-// transposed copy of E, h or d exists.  Tiles come by DMA (global_load_lds) into two
-// buffers, one barrier a 64-wide step; 16-byte chunks are XORed by row against bank
-// conflicts.
+// side).  h, E and d lie in panels of 32 columns (loss_layout copies h's rows and E once a
+// call); a tile comes by DMA (global_load_lds) into two buffers, one barrier a 32-wide step.
+// Operands whose k runs along a panel's rows are read from LDS as rows, others by transposing
+// reads (ds_read_b64_tr_b16), so no transposed copy exists.
+//
+// What bounds it: the operands' way from L2 (11 TB/s in loss_logits at 8192 rows; a third
+// less time with the copies left out, none with LDS reads or exp left out), and that a block's
+// waves wait together: three blocks a CU of 128 x 256 (165 registers) beat two of them with
+// deeper buffers (467 us against 491) and one of 256 x 256 (518).  Measured at 8192 rows, 49152
+// ids, 576 columns, bf16: logits 467 us (993 TFLOP/s), d 525, both gradients 1097 (846
+// TFLOP/s); the library's single products of these shapes take 539, 604 and 750.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -602,9 +608,14 @@ __global__ void __launch_bounds__(256) loss_dh_kernel(LossArgs a) {
   if (m >= 0) {
     const int rows = (a.cnt[0] + a.bl - 1) / a.bl * a.bl;
     const int splits = lk_splits(rows, rows / a.bl * a.nr, a);
-    for (int z = 0; z < splits; ++z) {
-      const float4 x = *reinterpret_cast<const float4*>(a.share + ((size_t)z * rows + m) * a.Hp + c);
-      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    for (int z0 = 0; z0 < splits; z0 += 8) {
+      float4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        x[k] = *reinterpret_cast<const float4*>(a.share + ((size_t)min(z0 + k, splits - 1) * rows + m) * a.Hp + c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (z0 + k < splits) s.x += x[k].x, s.y += x[k].y, s.z += x[k].z, s.w += x[k].w;
     }
     const float f = (a.mode == 2 ? a.gmax[0] : a.mode == 1 ? a.g[0] : a.g[0] / (float)a.cnt[0]) *
                     (BF ? 1.f : 1.f / LK_FP16);
