@@ -20,6 +20,7 @@ def main() -> int:
     p.add_argument("--steps", type=int, default=40)
     p.add_argument("--batch", type=int, default=128)
     p.add_argument("--fused", default="1,0", help="TrainConfig.fused values to measure (A/B)")
+    p.add_argument("--hip-ops", default="0", help="TrainConfig.hip_ops values to measure (A/B; needs fused)")
     a = p.parse_args()
     import torch
 
@@ -28,14 +29,15 @@ def main() -> int:
 
     tok = load_tokenizer()
     data = make_examples(tok, answer_fsm(tok, a.format), 8192, seed=1, negatives=0.12)
-    for fused in (bool(int(x)) for x in a.fused.split(",")):
+    values = [[bool(int(x)) for x in v.split(",")] for v in (a.fused, a.hip_ops)]
+    for fused, hip_ops in ((f, h) for f in values[0] for h in values[1] if f or not h):
         times = []
 
         def log(s):
             times.append((time.perf_counter(), s))
 
         tc = TrainConfig(steps=a.steps, batch=a.batch, n_examples=len(data), log_every=1, answer_format=a.format,
-                         warmup=5, fused=fused)
+                         warmup=5, fused=fused, hip_ops=hip_ops)
         train_extractor(tc, device="cuda", data=data, log=log)
         stamps = [t for t, s in times if s.startswith("step")]
         per = (stamps[-1] - stamps[10]) / (len(stamps) - 11) * 1e3
@@ -43,7 +45,7 @@ def main() -> int:
         from torch.profiler import ProfilerActivity, profile
 
         tc2 = TrainConfig(steps=6, batch=a.batch, n_examples=len(data), log_every=0, answer_format=a.format,
-                          warmup=2, fused=fused)
+                          warmup=2, fused=fused, hip_ops=hip_ops)
         with profile(activities=[ProfilerActivity.CUDA]) as prof:
             train_extractor(tc2, device="cuda", data=data, log=lambda s: None)
             torch.cuda.synchronize()
@@ -51,7 +53,7 @@ def main() -> int:
         kern = sum(e.count for e in kev)
         gpu_us = sum(e.self_device_time_total for e in kev)
         top = sorted(kev, key=lambda e: -e.self_device_time_total)[:12]
-        print(json.dumps({"format": a.format, "batch": a.batch, "fused": fused, "ms_per_step": round(per, 2),
+        print(json.dumps({"format": a.format, "batch": a.batch, "fused": fused, "hip_ops": hip_ops, "ms_per_step": round(per, 2),
                           "kernels_per_step": round(kern / 6, 1), "gpu_ms_per_step": round(gpu_us / 6 / 1e3, 2),
                           "top": [[e.key[:60], round(e.self_device_time_total / 6 / 1e3, 3), e.count // 6]
                                   for e in top]}), flush=True)
