@@ -276,7 +276,8 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch
     (``ids``' shape and type): a second row added to each position, negative = none (the
     span formats' pointer rows).  The sum is taken and scaled in fp32 and rounded once.  The
     table's gradient sums the positions of each id in fp32, in their order: the same bits
-    every run.  An id outside [0, V) (``add_ids``: above it) gives a NaN row and no gradient."""
+    every run.  An id outside [0, V) (``add_ids``: above it) makes its position NaN and has no row in
+    the gradient."""
     if table.dim() != 2 or table.dtype not in _DTYPES:
         raise TypeError("embed_lookup: table must be fp32, bf16 or fp16 [V, H]")
     if ids.dtype not in (torch.int32, torch.int64):
