@@ -404,7 +404,8 @@ __global__ void __launch_bounds__(NW * 64) attn_dq_kernel(AtArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, lse));
-        if (border.value && k0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h >= lim) p = 0.f;
+        // (a row of one key has P = 1 and dS = 0, not the rounding of dP - D)
+        if (border.value && (k0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h >= lim || lim == 1)) p = 0.f;
         ds[r] = BF ? p * dp[r] : p * dp[r] * dsf;
       }
 #pragma unroll
@@ -502,6 +503,7 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
         if (border.value && q0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h < kr) p[r] = 0.f;
         ds[r] = BF ? p[r] * dp[r] : p[r] * dp[r] * dsf;
       }
+      if (border.value && q0 == 0 && u == 0 && h == 0) ds[0] = 0.f;  // query 0 has one key: dS = 0
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const u16x8 pf = at_pack<BF>(p + 8 * e), sf = at_pack<BF>(ds + 8 * e);
@@ -527,6 +529,7 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
   if (kr >= a.T) return;
   const float fk = BF ? a.scale : a.scale / (dsf * (1 << AT_FP16_P));
   const float fv = BF ? 1.f : 1.f / (1 << AT_FP16_P);
+  const bool dkon = on && len > 1;  // (one key: dS = 0)
   const size_t row = ((size_t)bh * a.T + kr) * D;
   if (a.split) {
     float* pk = a.part + row;
@@ -537,17 +540,17 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
       for (int e = 0; e < 4; ++e) {
         const int d = 32 * dt + 8 * e + 4 * h;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (on) {
+        if (dkon)
           x = make_float4(dk[dt][4 * e] * fk, dk[dt][4 * e + 1] * fk, dk[dt][4 * e + 2] * fk, dk[dt][4 * e + 3] * fk);
+        if (on)
           y = make_float4(dv[dt][4 * e] * fv, dv[dt][4 * e + 1] * fv, dv[dt][4 * e + 2] * fv, dv[dt][4 * e + 3] * fv);
-        }
         *reinterpret_cast<float4*>(pk + d) = x;
         *reinterpret_cast<float4*>(pv + d) = y;
       }
   } else {
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
-      at_store<BF>(a.dk + row, dk[dt], fk, on, dt, h);
+      at_store<BF>(a.dk + row, dk[dt], fk, dkon, dt, h);
       at_store<BF>(a.dv + row, dv[dt], fv, on, dt, h);
     }
   }

@@ -10,8 +10,9 @@
 // once behind it (an SMS batch labels about a third of its positions).
 //
 //   forward   loss_logits<0>: a tile's logits stay in the accumulators; each row's maximum
-//             and sum of exponentials over the tile go out (8 bytes a row and tile);
-//             loss_join: L and loss, with z_i[y_i] as a dot product of its own
+//             and sum of exponentials over the tile go out (8 bytes a row and tile), the label's
+//             logit from the tile that has it;
+//             loss_join: L and loss
 //   backward  per piece of the vocabulary: loss_logits<1> recomputes the tile's logits and
 //             writes d in the inputs' type; loss_grad: the piece's rows of dE, and dh's
 //             shares, fp32, the piece's columns split over blocks; loss_dh sums the shares in
@@ -60,7 +61,7 @@ struct LossArgs {
   const void* labels;
   uint16_t *hc, *ec, *d, *dh, *dtable;  // hc, ec, d: panels
   int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; [1]
-  float *lse, *rl, *loss, *w;       // [Mp] L in log2; [Mp] loss; out; [Mp] row weights or null
+  float *lse, *rl, *loss, *w;       // [Mp] L; [Mp] label's logit, then loss; out; [Mp] row weights or null
   float2* part;                     // [v tiles][Mp] (maximum, sum of exp(z - maximum))
   float* share;                     // [splits][Mp][Hp]
   const float *g, *gmax;            // incoming gradient; none: its largest magnitude
@@ -91,14 +92,6 @@ __device__ __forceinline__ uint16_t lk_round(float x) {
     const _Float16 b = (_Float16)x;
     return __builtin_bit_cast(uint16_t, b);
   }
-}
-
-template <bool BF>
-__device__ __forceinline__ float lk_float(uint16_t x) {
-  if constexpr (BF)
-    return __uint_as_float((uint32_t)x << 16);
-  else
-    return (float)__builtin_bit_cast(_Float16, x);
 }
 
 template <bool BF>
@@ -374,6 +367,16 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
     const int vend = a.V - a.v0;
 #pragma unroll
     for (int j = 0; j < FL; ++j) {
+      // the label's logit, where this lane holds it: the same bits that the maximum and the
+      // sum are made of, so that a sure row's loss is 0 and not a rounding
+      const int n = ln + 32 * j, y = (n < cnt ? a.lab[n] : -1) - a.v0 - rn;
+      if (__any(y >= 0 && y < TR)) {
+#pragma unroll
+        for (int i = 0; i < FR; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (y == 32 * i + 8 * (r >> 2) + (r & 3)) a.rl[n] = acc[i][j][r];
+      }
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < FR; ++i)
@@ -417,7 +420,7 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
 #pragma unroll
       for (int i = 0; i < FR; ++i) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LK_LOG2E, -lse));
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = lk_exp(acc[i][j][r] - lse);
         if (__any(here)) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -489,11 +492,8 @@ __global__ void __launch_bounds__(WL * WR * 64, 3) loss_grad_kernel(LossArgs a) 
 
 // ---- joins -----------------------------------------------------------------------------
 // 16 rows a block: L from the tiles' (maximum, sum), the label's logit, the loss.
-template <bool BF>
 __global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
   __shared__ float2 red[16][16];
-  __shared__ float zy[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = blockIdx.x * 16, cnt = a.cnt[0];
   if (m0 >= cnt) return;
   const int r = threadIdx.x & 15, g = threadIdx.x >> 4;  // row, share of the tiles
@@ -515,31 +515,6 @@ __global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
     x = make_float2(top, s);
   }
   red[g][r] = x;
-  {  // z[y]: 4 rows a wave
-    const u16x8 *hr[4], *er[4];
-    float s[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int m = min(m0 + 4 * wave + k, cnt - 1);
-      hr[k] = reinterpret_cast<const u16x8*>(a.h + (size_t)a.rows[m] * a.H);
-      er[k] = reinterpret_cast<const u16x8*>(a.table + (size_t)max(a.lab[m], 0) * a.H);
-      s[k] = 0.f;
-    }
-    for (int c = lane; c < a.H / 8; c += 64) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const u16x8 p = hr[k][c], q = er[k][c];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[k] = fmaf(lk_float<BF>(p[e]), lk_float<BF>(q[e]), s[k]);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) s[k] += __shfl_xor(s[k], o, 64);
-      if (lane == 0) zy[4 * wave + k] = s[k];
-    }
-  }
   __syncthreads();
   const int m = m0 + threadIdx.x;
   if (threadIdx.x >= 16 || m >= cnt) return;
@@ -552,8 +527,8 @@ __global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
   for (int w = 0; w < 16; ++w) s += red[w][threadIdx.x].y * lk_exp(red[w][threadIdx.x].x - ref);
   float ls = __logf(s);
   if (a.lab[m] == -2) ls = __builtin_nanf("");
-  const float loss = (top - zy[threadIdx.x]) + ls;
-  a.lse[m] = (top + ls) * LK_LOG2E;
+  const float loss = (top - a.rl[m]) + ls;
+  a.lse[m] = top + ls;
   a.rl[m] = loss;
   if (a.mode == 2) a.loss[a.rows[m]] = loss;
 }
@@ -687,7 +662,7 @@ void lk_forward(LossArgs a, const LossPlan& p, hipStream_t st) {
   a.v0 = 0;
   a.vn = p.vtiles * (p.small ? 64 : 256);
   lk_logits<BF, 0>(a, p, st);
-  loss_join_kernel<BF><<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
+  loss_join_kernel<<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
   if (a.mode != 2) loss_sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
 }
 

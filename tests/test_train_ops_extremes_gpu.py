@@ -103,6 +103,47 @@ def test_ignored_rows_may_hold_anything():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_one_key_has_no_gradient(dtype, causal):
+    """A row that sees one key: P = 1, so dq and dk are 0, not what rounding leaves of dP - D."""
+    from smsgate_amd.models import train_ops
+
+    g = torch.Generator(device=dev).manual_seed(6)
+    for T, lens in ((1, None), (70, [1, 1, 0]), (200, [1, 1, 1])):
+        q, k, v = (torch.randn(3, h, T, 64, generator=g, device=dev).to(dtype).requires_grad_() for h in (6, 2, 2))
+        lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev)
+        out = train_ops.tiled_attention(q, k, v, causal=causal, lengths=lengths)
+        dq, dk, dv = torch.autograd.grad(out, (q, k, v), torch.randn(out.shape, generator=g, device=dev).to(dtype))
+        assert not dq.any() and not dk.any() and dv.any()
+        n = 1 if lens is None else lens[0]
+        assert torch.equal(out[0, :n].reshape(n, 6, 64), v[0, :, :n].transpose(0, 1).repeat_interleave(3, 1))
+    q, k, v = (torch.randn(1, h, 100, 64, generator=g, device=dev).to(dtype).requires_grad_() for h in (6, 2, 2))
+    out = train_ops.tiled_attention(q, k, v)
+    (dq,) = torch.autograd.grad(out, q, torch.ones_like(out))
+    assert not dq[:, :, 0].any() and dq[:, :, 1].any()
+
+
+def test_sure_rows_lose_nothing():
+    """The label's logit far above all others (or alone): the loss and the gradients are 0."""
+    from smsgate_amd.models import train_ops
+
+    g = torch.Generator(device=dev).manual_seed(8)
+    for V, N in ((1, 5), (600, 200), (9000, 2100)):
+        table = torch.randn(V, 64, generator=g, device=dev)
+        table = (table / table.norm(dim=1, keepdim=True)).bfloat16()
+        labels = torch.randint(0, V, (N,), generator=g, device=dev)
+        h = (table[labels].float() * 900).bfloat16().requires_grad_()  # ahead by 900 (1 - cos)
+        table.requires_grad_()
+        each = train_ops.lm_loss(h, table, labels, reduction="none")
+        far = (h.double() @ table.double().t()).topk(min(2, V), 1).values
+        sure = torch.ones(N, dtype=torch.bool, device=dev) if V == 1 else far[:, 0] - far[:, 1] > 110.0
+        assert sure.float().mean() > 0.9
+        assert not each[sure].any()
+        dh, dt = torch.autograd.grad(each, (h, table), sure.float())
+        assert not dh.any() and not dt.any()
+
+
 def _calls():
     """(name, leaves, a call of them) of each operator, small enough to be launched together."""
     from smsgate_amd.models import train_ops
