@@ -34,7 +34,7 @@
 // (another value of the type), so that D is taken from 16 more bits of o: from the rounded o
 // alone its error was a third of dq's and dk's (2.8e-3 instead of 2.3e-3 of their norm at
 // 61 rows, bf16).  P and dS are rounded to the inputs' type as
-// operands (relative 2^-9 each, as the inputs themselves are).  fp16 holds no value under
+// operands (at most 2^-8 relative in bf16, as the inputs themselves are; see at_mma_p).  fp16 holds no value under
 // 2^-24: there P is scaled by 2^8 and dS by a power of two that the largest |do| sets.
 //
 // What bounds it: the waves' own chains (product, exp2, rounding, product): at 16384 rows the
@@ -183,6 +183,26 @@ __device__ __forceinline__ u16x8 at_pack(const float* p) {
   return r;
 }
 
+// Eight values of P or dS as operands: rounded, and (FINE) what rounding took as a second
+// product.  A result carries its terms' roundings besides its own: 2.4e-3 of its norm off in
+// bf16 for 1.7e-3, and where few rows are summed 2.7e-3.  FINE is for those, dS up to 64 rows
+// (dq and dk 1.9e-3; 128 x 61 rows take 41.7 us with it for 40.1), P up to 32 (out and dv as
+// near as their type allows; up to 64 rows it takes 1.4 us more, and they stay under 2.3e-3).
+template <bool BF, bool FINE, int DT>
+__device__ __forceinline__ void at_mma_p(f32x16 (&o)[DT], const u16x8 (&col)[DT], const float* p) {
+  const u16x8 hi = at_pack<BF>(p);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = at_mma<BF>(col[dt], hi, o[dt]);
+  if constexpr (FINE) {
+    float r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = p[j] - at_float<BF>(hi[j]);
+    const u16x8 lo = at_pack<BF>(r);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = at_mma<BF>(col[dt], lo, o[dt]);
+  }
+}
+
 __device__ __forceinline__ void at_wait() {
   // this wave's DMAs have landed and its reads of the other buffer are done ...
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -288,10 +308,10 @@ __global__ void __launch_bounds__(NW * 64) attn_fwd_kernel(AtArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const u16x8 pf = at_pack<BF>(p + 8 * e);
+        u16x8 vc[D / 32];
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-          o[dt] = at_mma<BF>(at_col<D>(vs, 32 * u + 16 * e, dt, lane), pf, o[dt]);
+        for (int dt = 0; dt < D / 32; ++dt) vc[dt] = at_col<D>(vs, 32 * u + 16 * e, dt, lane);
+        at_mma_p<BF, NW == 1, D / 32>(o, vc, p + 8 * e);
       }
     }
   }
@@ -410,10 +430,10 @@ __global__ void __launch_bounds__(NW * 64) attn_dq_kernel(AtArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const u16x8 pf = at_pack<BF>(ds + 8 * e);
+        u16x8 kc[D / 32];
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-          dq[dt] = at_mma<BF>(at_col<D>(ks, 32 * u + 16 * e, dt, lane), pf, dq[dt]);
+        for (int dt = 0; dt < D / 32; ++dt) kc[dt] = at_col<D>(ks, 32 * u + 16 * e, dt, lane);
+        at_mma_p<BF, NW <= 2, D / 32>(dq, kc, ds + 8 * e);
       }
     }
   };
@@ -506,12 +526,14 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
       if (border.value && q0 == 0 && u == 0 && h == 0) ds[0] = 0.f;  // query 0 has one key: dS = 0
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const u16x8 pf = at_pack<BF>(p + 8 * e), sf = at_pack<BF>(ds + 8 * e);
+        u16x8 oc[D / 32], qc[D / 32];
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) {
-          dv[dt] = at_mma<BF>(at_col<D>(os, 32 * u + 16 * e, dt, lane), pf, dv[dt]);
-          dk[dt] = at_mma<BF>(at_col<D>(qs, 32 * u + 16 * e, dt, lane), sf, dk[dt]);
+          oc[dt] = at_col<D>(os, 32 * u + 16 * e, dt, lane);
+          qc[dt] = at_col<D>(qs, 32 * u + 16 * e, dt, lane);
         }
+        at_mma_p<BF, NW == 1, D / 32>(dv, oc, p + 8 * e);
+        at_mma_p<BF, NW <= 2, D / 32>(dk, qc, ds + 8 * e);
       }
     }
   };
