@@ -30,6 +30,10 @@ Three operators of the whole step, on request (``hip_ops``; TrainConfig.hip_ops)
 * :func:`lm_loss`: cross entropy over the embedding's rows without logits, for the copy and
   span answer formats (csrc/loss_kernels.hip).
 
+Their forward and backward can be captured into a graph.  As with any torch operator, no
+eager graph of the same leaves may be alive then: a leaf's accumulation node belongs to the
+stream that it was first used on, and autograd waits for that stream inside the capture.
+
 GEMMs stay hipBLASLt (autocast bf16), so the math is
 reference_forward's up to bf16 rounding order (tests/test_train_ops_gpu.py compares
 losses and gradients).  CPU / no-library: reference_forward.
@@ -284,8 +288,8 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch
         raise TypeError("embed_lookup: ids must be int32 or int64")
     if add_ids is not None and (add_ids.shape != ids.shape or add_ids.dtype != ids.dtype):
         raise ValueError("embed_lookup: add_ids must have the shape and type of ids")
-    if not (1 <= table.shape[0] < 1 << 30 and 1 <= table.shape[1] <= 1 << 20) or ids.numel() >= 1 << 29:
-        raise ValueError("embed_lookup: 1 <= V < 2^30, 1 <= H <= 2^20, fewer than 2^29 ids")
+    if not (1 <= table.shape[0] < 1 << 26 and 1 <= table.shape[1] <= 1 << 20) or ids.numel() >= 1 << 26:
+        raise ValueError("embed_lookup: 1 <= V < 2^26, 1 <= H <= 2^20, fewer than 2^26 ids")
     _on_gpu("embed_lookup", table, ids, add_ids)
     return _Embed.apply(table, ids, add_ids, float(scale))
 
@@ -297,7 +301,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous and on a 16-byte border (a copy where it is not)."""
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -305,7 +309,7 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     b, h, r, c = t.stride()
     if c == 1 and (b | h | r) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
-    return t.contiguous() if c != 1 or (b | h | r) % 8 else t.clone(memory_format=torch.contiguous_format)
+    return _aligned(t)
 
 
 @functools.lru_cache(maxsize=256)
@@ -313,7 +317,7 @@ def _attn_plan(B: int, T: int, nh: int, nkv: int, D: int, fp16: int):
     """32-bit words of the row statistics and of the backward's workspace."""
     lib = _lib()
     stats = B * nh * lib.sg_attn_rows(T)
-    return stats, stats + 256 * fp16 + (2 * B * nh * T * D if lib.sg_attn_split(B, T, nh, nkv) else 0)
+    return stats, stats + 512 * fp16 + (2 * B * nh * T * D if lib.sg_attn_split(B, T, nh, nkv) else 0)
 
 
 class _TiledAttention(torch.autograd.Function):
@@ -376,11 +380,11 @@ def tiled_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
     B, nh, T, D = q.shape
     if k.shape[0] != B or k.shape[2:] != (T, D) or nh % k.shape[1] or D not in (64, 128):
         raise ValueError("tiled_attention: k and v need q's batch, length and width (64 or 128), and nh % nkv == 0")
-    if T > 1 << 24 or B * nh > 1 << 20 or B * nh * ((T + 31) // 32) > 0x7FFFFFFF:
-        raise ValueError("tiled_attention: T <= 2^24, B * nh <= 2^20, fewer than 2^31 tiles")
+    if T > 1 << 24 or B * nh > 1 << 20 or B * nh * ((T + 127) // 128) >= 1 << 24:
+        raise ValueError("tiled_attention: T <= 2^24, B * nh <= 2^20, fewer than 2^24 tiles of 128 rows")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError("tiled_attention: scale must be finite and above 0")
+    if not 1e-30 < scale < 1e30:
+        raise ValueError("tiled_attention: scale must be finite and above 0 (1e-30 to 1e30)")
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,)):
         raise ValueError("tiled_attention: lengths must be int32 [B]")
     _on_gpu("tiled_attention", q, k, v, lengths)
@@ -460,8 +464,9 @@ def lm_loss(h: torch.Tensor, table: torch.Tensor, labels: torch.Tensor, *, reduc
     V, H = table.shape
     N = labels.numel()
     if not (1 <= N <= 1 << 24 and 1 <= V <= 1 << 24 and 8 <= H <= 1 << 14) or H % 8 \
-            or ((N + 255) // 64) * ((V + 255) // 64) > 0x7FFFFFFF:
-        raise ValueError("lm_loss: 1 to 2^24 rows and ids, H a multiple of 8 up to 2^14, fewer than 2^31 tiles")
+            or ((N + 255) // 128) * ((V + 255) // 256) >= 1 << 24 or (N + V + 512) * (H + 63) >= 1 << 34:
+        raise ValueError("lm_loss: 1 to 2^24 rows and ids, H a multiple of 8 up to 2^14, fewer than 2^24 tiles of "
+                         "128 x 256, (rows + ids) * H under 2^34")
     if not -(1 << 31) <= ignore_index < 1 << 31:
         raise ValueError("lm_loss: ignore_index must fit 32 bits")
     _on_gpu("lm_loss", h, table, labels)

@@ -35,7 +35,7 @@
 // alone its error was a third of dq's and dk's (2.8e-3 instead of 2.3e-3 of their norm at
 // 61 rows, bf16).  P and dS are rounded to the inputs' type as
 // operands (at most 2^-8 relative in bf16, as the inputs themselves are; see at_mma_p).  fp16 holds no value under
-// 2^-24: there P is scaled by 2^8 and dS by a power of two that the largest |do| sets.
+// 2^-24: there P is scaled by 2^8 and dS by a power of two that the longest rows of do and v set.
 //
 // What bounds it: the waves' own chains (product, exp2, rounding, product): at 16384 rows the
 // matrix units work a third of the time, the vector units half, and neither copies (10 % less
@@ -61,7 +61,7 @@ typedef __attribute__((address_space(3))) s16x4* at_tr_t;
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr float AT_LN2 = 0.6931471805599453f;
 constexpr int AT_FP16_P = 8;    // fp16: log2 of the factor on P in attn_dkv
-constexpr int AT_MAXPARTS = 256;  // fp16: blocks of the |do| maximum
+constexpr int AT_MAXPARTS = 256;  // fp16: blocks of each maximum
 
 __device__ const uint4 at_zero = {0, 0, 0, 0};  // what rows outside a sequence are read as
 
@@ -69,7 +69,7 @@ struct AtArgs {
   const uint16_t *q, *k, *v, *o, *dout;
   uint16_t *out, *olo, *dq, *dk, *dv;  // olo: what rounding took from o, or null (no backward)
   float *lse, *dsum, *part;   // [B, nh, Tp]: -L in log2, -D; [B, nh, T, D] x 2: dk, dv by query head
-  const float* omax;          // fp16: AT_MAXPARTS maxima of |do|
+  const float* omax;          // fp16: AT_MAXPARTS maxima of |do|^2, as many of |v|^2
   const int* lens;            // [B] or null
   long qb, qh, qt, kb, kh, kt, vb, vh, vt;  // strides in elements
   int B, T, Tp, nh, nkv, causal, split;
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(NW * 64) attn_fwd_kernel(AtArgs a) {
   f32x16 o[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = (f32x16)0.f;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, ref = 0.f, l = 0.f;  // ref: m, or 0 while every S is -infinity
   const float c = a.scale * AT_LOG2E;
   auto stage = [&](int t) {
     uint16_t* dst = sm + (t & 1) * 2 * TILE;
@@ -288,10 +288,14 @@ __global__ void __launch_bounds__(NW * 64) attn_fwd_kernel(AtArgs a) {
       top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][r]), s[1][r]);
     top = at_max_halves(top) * c;
     // any reference value serves the softmax: m follows the maximum only when it rises by
-    // over 2^8, so most tiles skip the rescaling of o
-    if (__any(top > m + 8.f)) {
-      const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
+    // over 2^8, so most tiles skip the rescaling of o.  fp16: the reference lies 2^7 below,
+    // so that P (at most 2^15) loses less under fp16's 2^-24
+    constexpr float LOW = BF ? 0.f : 7.f;
+    if (__any(top > m + (8.f + LOW))) {
+      const float was = m;
+      m = fmaxf(m, top - LOW);
+      ref = m == -INFINITY ? 0.f : m;
+      const float f = __builtin_amdgcn_exp2f(was - ref);
       l *= f;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(NW * 64) attn_fwd_kernel(AtArgs a) {
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -m));
+        p[r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -ref));
         l += p[r];
       }
 #pragma unroll
@@ -336,31 +340,67 @@ __global__ void __launch_bounds__(NW * 64) attn_fwd_kernel(AtArgs a) {
   if (h == 0 && qr < a.Tp) a.lse[(size_t)bh * a.Tp + qr] = on ? -(m + __log2f(l)) : -INFINITY;
 }
 
-// fp16: the factor on dS, 16 / 2^floor(log2 max|do|)
+// fp16: the factor on dS.  dS = P (dP - D) where D is the mean of dP, so |dS| is at most half
+// of the largest |dP|, and that at most |do| |v| over the longest rows of both: the factor
+// takes this bound to 2^15, under fp16's 65504.
 __device__ __forceinline__ float at_ds_factor(const float* omax, int lane) {
-  float x = 0.f;
+  float x = 0.f, y = 0.f;
 #pragma unroll
-  for (int i = 0; i < AT_MAXPARTS / 64; ++i) x = fmaxf(x, omax[lane + 64 * i]);
+  for (int i = 0; i < AT_MAXPARTS / 64; ++i) {
+    x = fmaxf(x, omax[lane + 64 * i]);
+    y = fmaxf(y, omax[AT_MAXPARTS + lane + 64 * i]);
+  }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-  if (!(x > 0.f) || x > 65504.f) return 1.f;
-  return __uint_as_float((254u << 23) - (__float_as_uint(x) & 0x7f800000u)) * 16.f;
+  for (int o = 32; o > 0; o >>= 1) {
+    x = fmaxf(x, __shfl_xor(x, o, 64));
+    y = fmaxf(y, __shfl_xor(y, o, 64));
+  }
+  x *= y;
+  if (!(x > 0.f && x < 1e30f)) return 1.f;
+  const int e = (int)(__float_as_uint(x) >> 23) - 127;  // |do| |v| < 2^(e / 2 rounded down + 1)
+  return __uint_as_float((uint32_t)(127 + 15 - (e >> 1)) << 23);
 }
 
-__global__ void __launch_bounds__(256) attn_omax_kernel(const uint16_t* __restrict__ x, long n8,
-                                                        float* __restrict__ omax) {
-  __shared__ float red[4];
+// The largest squared length of do's (y = 0) and v's (y = 1) rows of a head inside the
+// sequences: what lies behind them must not move the factor.  D / 8 lanes a row.
+template <int D>
+__global__ void __launch_bounds__(1024) attn_omax_kernel(AtArgs a) {
+  __shared__ float red[16];
+  const bool isv = blockIdx.y == 1;
+  const int heads = isv ? a.nkv : a.nh;
+  const long rows = (long)heads * a.T, n = a.B * rows * (D / 8);
+  // (64-bit divisions cost most of the kernel; almost every batch does without)
+  auto div = [&](long x, long y) { return n >> 32 ? x / y : (long)((uint32_t)x / (uint32_t)y); };
   float m = 0.f;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n8; i += (long)gridDim.x * 256) {
-    const f16x8 v = reinterpret_cast<const f16x8*>(x)[i];
+  for (long i = (long)blockIdx.x * 1024 + threadIdx.x; i < n; i += (long)AT_MAXPARTS * 1024) {
+    const long r = i / (D / 8), b = div(r, rows), j = r - b * rows;
+    const int c = (int)(i % (D / 8)) * 8;
+    const int len = a.lens != nullptr ? min(max(a.lens[b], 0), a.T) : a.T;
+    const uint16_t* p;
+    if (isv) {
+      const long g = div(j, a.T), t = j - g * a.T;
+      if (t >= len) continue;
+      p = a.v + b * a.vb + g * a.vh + t * a.vt + c;
+    } else {
+      if (j >= (long)len * heads) continue;
+      p = a.dout + r * D + c;
+    }
+    const f16x8 v = *reinterpret_cast<const f16x8*>(p);
+    float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf((float)v[j]));
+    for (int k = 0; k < 8; ++k) s = fmaf((float)v[k], (float)v[k], s);
+#pragma unroll
+    for (int o = 1; o < D / 8; o <<= 1) s += __shfl_xor(s, o, 64);
+    m = fmaxf(m, s);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) omax[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w]);
+    const_cast<float*>(a.omax)[blockIdx.y * AT_MAXPARTS + blockIdx.x] = m;
+  }
 }
 
 template <bool BF, int D, int NW>
@@ -602,7 +642,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const float* __restrict_
 
 bool at_bad(int B, int T, int nh, int nkv, int D) {
   return B <= 0 || T <= 0 || T > (1 << 24) || nkv <= 0 || nh <= 0 || nh % nkv != 0 || (D != 64 && D != 128) ||
-         (long)B * nh > (1 << 20) || ((long)T + 31) / 32 * B * nh > 0x7fffffffL;
+         (long)B * nh > (1 << 20) || ((long)T + 127) / 128 * B * nh >= 1 << 24;  // (a grid holds 2^32 threads)
 }
 
 template <bool BF, int D>
@@ -619,9 +659,7 @@ void at_launch_fwd(const AtArgs& a, hipStream_t st) {
 template <bool BF, int D>
 void at_launch_bwd(const AtArgs& a, hipStream_t st) {
   const int pairs = a.B * a.nh, kpairs = a.B * (a.split ? a.nh : a.nkv);
-  if constexpr (!BF)
-    attn_omax_kernel<<<dim3(AT_MAXPARTS), dim3(256), 0, st>>>(a.dout, (long)a.B * a.T * a.nh * D / 8,
-                                                              const_cast<float*>(a.omax));
+  if constexpr (!BF) attn_omax_kernel<D><<<dim3(AT_MAXPARTS, 2), dim3(1024), 0, st>>>(a);
   if (a.T <= 32) {
     attn_dq_kernel<BF, D, 1><<<dim3((a.Tp + 31) / 32 * pairs), dim3(64), 0, st>>>(a);
     attn_dkv_kernel<BF, D, 1><<<dim3((a.T + 31) / 32 * kpairs), dim3(64), 0, st>>>(a);
@@ -668,7 +706,7 @@ int sg_attn_fwd(const void* q, const void* k, const void* v, const void* lens, v
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-// ws: fp32 [B nh rows] (D), then 256 (fp16 only), then [2][B, nh, T, D] where sg_attn_split
+// ws: fp32 [B nh rows] (D), then 512 (fp16 only), then [2][B, nh, T, D] where sg_attn_split
 int sg_attn_bwd(const void* q, const void* k, const void* v, const void* lens, const void* out, const void* olo,
                 const void* lse, const void* dout, void* dq, void* dk, void* dv, void* ws, const void* strides, int B, int T, int nh,
                 int nkv, int D, int causal, int fp16, float scale, hipStream_t st) {
@@ -685,7 +723,7 @@ int sg_attn_bwd(const void* q, const void* k, const void* v, const void* lens, c
   float* w = a.dsum + (size_t)B * nh * a.Tp;
   if (fp16) {
     a.omax = w;
-    w += AT_MAXPARTS;
+    w += 2 * AT_MAXPARTS;
   }
   a.part = w;
   if (fp16)

@@ -515,6 +515,12 @@ int eg_backward(const void* ids, const void* add, int is64, const void* dx, void
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
+// (a grid holds 2^32 threads: 64 a row of x, 64 a row of dE)
+bool eg_bad(int n, int V, int H, int dtype, int vec) {
+  return n <= 0 || n >= (1 << 26) || V <= 0 || V >= (1 << 26) || H <= 0 || H > (1 << 20) || dtype < 0 || dtype > 2 ||
+         (vec && H % (dtype == 0 ? 4 : 8));
+}
+
 }  // namespace
 
 extern "C" {
@@ -522,7 +528,7 @@ extern "C" {
 // dtype 0 fp32, 1 bf16, 2 fp16; vec: every pointer and row is a multiple of 16 bytes
 int sg_embed_fwd(const void* ids, const void* add, int is64, const void* table, void* x, int n, int V, int H,
                  float scale, int dtype, int vec, hipStream_t st) {
-  if (n <= 0 || V <= 0 || H <= 0 || dtype < 0 || dtype > 2 || (vec && H % (dtype == 0 ? 4 : 8))) return 1;
+  if (eg_bad(n, V, H, dtype, vec)) return 1;
   if (dtype == 0)
     return vec ? eg_forward<float, 4>(ids, add, is64, table, x, n, V, H, scale, st)
                : eg_forward<float, 1>(ids, add, is64, table, x, n, V, H, scale, st);
@@ -542,9 +548,7 @@ int sg_embed_grad_ws(int n2, int V, int H) {
 
 int sg_embed_grad(const void* ids, const void* add, int is64, const void* dx, void* dt, int n, int V, int H,
                   float scale, int dtype, int vec, void* ws, int ws_units, hipStream_t st) {
-  if (n <= 0 || V <= 0 || V >= (1 << 30) || H <= 0 || n > (1 << 30) - 1 || dtype < 0 || dtype > 2 ||
-      (vec && H % (dtype == 0 ? 4 : 8)))
-    return 1;
+  if (eg_bad(n, V, H, dtype, vec)) return 1;
   const int n2 = add != nullptr ? 2 * n : n;
   uint32_t* keys = nullptr;
   int* ents = nullptr;

@@ -126,7 +126,7 @@ __device__ __forceinline__ float lk_exp(float x) { return __builtin_amdgcn_exp2f
 __device__ __forceinline__ float lk_exp_fine(float x) {
   const float t = x * LK_LOG2E, lo = fmaf(x, 1.92596303e-8f, fmaf(x, LK_LOG2E, -t));
   const float e = __builtin_amdgcn_exp2f(t);
-  return x == -INFINITY ? 0.f : fmaf(e, lo * 0.693147181f, e);
+  return x < -150.f ? 0.f : fmaf(e, lo * 0.693147181f, e);  // (-infinity would give NaN)
 }
 
 __device__ __forceinline__ float4 lk_four(const f32x16& x, int e, float f) {
@@ -563,12 +563,15 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(LossArgs a) {
   if (threadIdx.x == 0) a.loss[0] = a.mode == 0 ? s / (float)cnt : s;
 }
 
-// none: w = g / max |g| (in [-1, 1]), gmax
+// none: gmax = the largest finite |g|, w = g / gmax (in [-1, 1])
 __global__ void __launch_bounds__(1024) loss_weights_kernel(LossArgs a, float* gmax) {
   __shared__ float red[16];
   const int cnt = a.cnt[0], lane = threadIdx.x & 63;
   float t = 0.f;
-  for (int m = threadIdx.x; m < cnt; m += 1024) t = fmaxf(t, fabsf(a.g[a.rows[m]]));
+  for (int m = threadIdx.x; m < cnt; m += 1024) {
+    const float x = fabsf(a.g[a.rows[m]]);
+    if (x < INFINITY) t = fmaxf(t, x);  // (an infinite or NaN g is its own row's matter)
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
   if (lane == 0) red[threadIdx.x >> 6] = t;
@@ -694,7 +697,8 @@ void lk_backward(LossArgs a, const LossPlan& p, hipStream_t st) {
 
 bool lk_bad(int N, int V, int H, int mode) {
   return N <= 0 || N > (1 << 24) || V <= 0 || V > (1 << 24) || H <= 0 || H % 8 != 0 || H > (1 << 14) || mode < 0 ||
-         mode > 2 || ((long)N + 255) / 64 * (((long)V + 255) / 64) > 0x7fffffffL;
+         // a grid holds 2^32 threads: 256 a tile of 128 x 256, one for 16 bytes of hc, ec or dh
+         mode > 2 || ((long)N + 255) / 128 * (((long)V + 255) / 256) >= 1 << 24 || ((long)N + V + 512) * (H + 63) >= 1L << 34;
 }
 
 // state: ints pos[N], rows[Mp], lab[Mp], cnt[64]; floats lse[Mp], rl[Mp]
