@@ -30,6 +30,10 @@ Three operators of the whole step, on request (``hip_ops``; TrainConfig.hip_ops)
 * :func:`lm_loss`: cross entropy over the embedding's rows without logits, for the copy and
   span answer formats (csrc/loss_kernels.hip).
 
+Their autograd functions are C++ (csrc/train_autograd.cpp): one message's call is host time,
+and a Python Function spends 1.4 times as much of it (45 positions forward and backward 37 ->
+27 us, attention of 37 rows 59 -> 42, the loss of 61 rows 70 -> 57).
+
 Their forward and backward can be captured into a graph.  As with any torch operator, no
 eager graph of the same leaves may be alive then: a leaf's accumulation node belongs to the
 stream that it was first used on, and autograd waits for that stream inside the capture.
@@ -41,7 +45,6 @@ losses and gradients).  CPU / no-library: reference_forward.
 from __future__ import annotations
 
 import contextlib
-import ctypes
 import functools
 import math
 import os
@@ -49,7 +52,6 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from .. import ops
 from .extractor import ExtractorWeights, _rope_tables
@@ -203,19 +205,19 @@ class _Attention(torch.autograd.Function):
         return dq, dk, dv, None
 
 
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # csrc/embed_kernels.hip
+_TABLES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _run(dev: int, name: str, fn, *args) -> None:
-    """Launches ``fn`` on device ``dev`` (current or not), on that device's current stream
-    (its raw handle: a Stream object costs as much host time as the launch)."""
-    if dev == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if rc != 0:
-        raise RuntimeError(f"{name} failed (rc={rc})")
+@functools.lru_cache(maxsize=1)
+def _native():
+    """The operators' autograd functions (csrc/train_autograd.cpp)."""
+    return ops.load_train_autograd()
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [B, heads, T, D] itself when its rows can be read 16 bytes at a time, else a copy
+    (what tiled_attention does with q, k and v)."""
+    return _native().rows16(t)
 
 
 def _on_gpu(name: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -223,52 +225,6 @@ def _on_gpu(name: str, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and (not t.is_cuda or t.device != first.device):
             raise ValueError(f"{name}: every tensor must be on the same GPU")
-
-
-def _vec16(H: int, *tensors: torch.Tensor) -> int:
-    """1 when rows of ``H`` elements of every tensor can be read 16 bytes at a time."""
-    ptrs = 0
-    for t in tensors:
-        ptrs |= t.data_ptr()
-    return int((ptrs | H * tensors[0].element_size()) % 16 == 0)
-
-
-@functools.lru_cache(maxsize=256)
-def _embed_units(entries: int, V: int, H: int) -> int:
-    return _lib().sg_embed_grad_ws(entries, V, H)
-
-
-class _Embed(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table: torch.Tensor, ids: torch.Tensor, add: Optional[torch.Tensor], scale: float):
-        V, H = table.shape
-        n, dev, code, is64 = ids.numel(), table.get_device(), _DTYPES[table.dtype], int(ids.dtype == torch.int64)
-        table, ids = table.contiguous(), ids.contiguous()
-        add = None if add is None else add.contiguous()
-        x = torch.empty(*ids.shape, H, dtype=table.dtype, device=table.device)
-        lib = _lib()
-        if n:
-            _run(dev, "embed_fwd", lib.sg_embed_fwd, ids.data_ptr(), ops._p(add), is64, table.data_ptr(),
-                 x.data_ptr(), n, V, H, scale, code, _vec16(H, table, x))
-        ctx.save_for_backward(ids, add)
-        # all that the gradient's launch needs but the pointers: autograd's thread pays
-        # more for each Python step than the caller's
-        ctx.plan = (lib.sg_embed_grad, dev, n, V, H, scale, code, is64, _embed_units(n if add is None else 2 * n, V, H))
-        return x
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dx: torch.Tensor):
-        fn, dev, n, V, H, scale, code, is64, units = ctx.plan
-        if not n:
-            return dx.new_zeros(V, H), None, None, None
-        ids, add = ctx.saved_tensors
-        dx = dx.contiguous()
-        dt = dx.new_empty(V, H)
-        ws = dx.new_empty(units * 64, dtype=torch.int32) if units else None  # units of 256 bytes
-        _run(dev, "embed_grad", fn, ids.data_ptr(), ops._p(add), is64, dx.data_ptr(), dt.data_ptr(), n, V, H, scale,
-             code, _vec16(H, dx, dt), ops._p(ws), units)
-        return dt, None, None, None
 
 
 def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch.Tensor] = None, *,
@@ -282,7 +238,7 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch
     table's gradient sums the positions of each id in fp32, in their order: the same bits
     every run.  An id outside [0, V) (``add_ids``: above it) makes its position NaN and has no row in
     the gradient."""
-    if table.dim() != 2 or table.dtype not in _DTYPES:
+    if table.dim() != 2 or table.dtype not in _TABLES:
         raise TypeError("embed_lookup: table must be fp32, bf16 or fp16 [V, H]")
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError("embed_lookup: ids must be int32 or int64")
@@ -291,73 +247,11 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch
     if not (1 <= table.shape[0] < 1 << 26 and 1 <= table.shape[1] <= 1 << 20) or ids.numel() >= 1 << 26:
         raise ValueError("embed_lookup: 1 <= V < 2^26, 1 <= H <= 2^20, fewer than 2^26 ids")
     _on_gpu("embed_lookup", table, ids, add_ids)
-    return _Embed.apply(table, ids, add_ids, float(scale))
+    return _native().embed(table, ids, add_ids, float(scale))
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -> torch.Tensor:
     return _Attention.apply(q, k, v, scale)
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and on a 16-byte border (a copy where it is not)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [B, heads, T, D] itself when its rows can be read 16 bytes at a time, else a copy."""
-    b, h, r, c = t.stride()
-    if c == 1 and (b | h | r) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return _aligned(t)
-
-
-@functools.lru_cache(maxsize=256)
-def _attn_plan(B: int, T: int, nh: int, nkv: int, D: int, fp16: int):
-    """32-bit words of the row statistics and of the backward's workspace."""
-    lib = _lib()
-    stats = B * nh * lib.sg_attn_rows(T)
-    return stats, stats + 512 * fp16 + (2 * B * nh * T * D if lib.sg_attn_split(B, T, nh, nkv) else 0)
-
-
-class _TiledAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, lengths, scale: float, causal: bool):
-        B, nh, T, D = q.shape
-        nkv, dev, fp16 = k.shape[1], q.get_device(), int(q.dtype == torch.float16)
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        if lengths is not None:
-            lengths = lengths.contiguous()
-        lib = _lib()
-        stats, words = _attn_plan(B, T, nh, nkv, D, fp16)
-        out = torch.empty(B, T, nh * D, dtype=q.dtype, device=q.device)
-        # the rows' statistics, and behind them what rounding took from out, for the
-        # backward's D (not where no gradient will be asked for)
-        grad = any(ctx.needs_input_grad[:3])
-        keep = torch.empty(stats + (B * T * nh * D // 2 if grad else 0), dtype=torch.float32, device=q.device)
-        lse = keep.data_ptr()
-        olo = lse + 4 * stats if grad else None
-        strides = (ctypes.c_long * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-        dims = (B, T, nh, nkv, D, int(causal), fp16, scale)
-        _run(dev, "attn_fwd", lib.sg_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), ops._p(lengths),
-             out.data_ptr(), olo, lse, strides, *dims)
-        ctx.save_for_backward(q, k, v, lengths, out, keep)
-        ctx.plan = (lib.sg_attn_bwd, dev, strides, dims, stats, words)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout: torch.Tensor):
-        q, k, v, lengths, out, keep = ctx.saved_tensors
-        fn, dev, strides, dims, stats, words = ctx.plan
-        dout = _aligned(dout)
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        ws = keep.new_empty(words)
-        lse = keep.data_ptr()
-        _run(dev, "attn_bwd", fn, q.data_ptr(), k.data_ptr(), v.data_ptr(), ops._p(lengths), out.data_ptr(),
-             lse + 4 * stats, lse, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), strides,
-             *dims)
-        return dq, dk, dv, None, None, None
 
 
 def tiled_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None, *,
@@ -388,56 +282,10 @@ def tiled_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,)):
         raise ValueError("tiled_attention: lengths must be int32 [B]")
     _on_gpu("tiled_attention", q, k, v, lengths)
-    return _TiledAttention.apply(q, k, v, lengths, scale, bool(causal))
+    return _native().attention(q, k, v, lengths, scale, bool(causal))
 
 
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
-
-
-@functools.lru_cache(maxsize=256)
-def _loss_plan(N: int, V: int, H: int):
-    """Elements of hc, ec and state (in the inputs' 16 bits), 32-bit words of the forward's and
-    the backward's workspace."""
-    plan = (ctypes.c_int * 6)()
-    _ok(_lib().sg_loss_plan(N, V, H, plan), "loss_plan")
-    rows, cols, vrows, state, fwd, bwd = plan
-    return rows * cols, vrows * cols, state * 128, fwd * 64, bwd * 64
-
-
-class _LmLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, h, table, labels, mode: int, ignore: int):
-        V, H = table.shape
-        N, dev, fp16 = labels.numel(), h.get_device(), int(h.dtype == torch.float16)
-        shape, h, table, labels = h.shape, _aligned(h), _aligned(table), labels.contiguous()
-        lib = _lib()
-        nhc, nec, nst, fwd, bwd = _loss_plan(N, V, H)
-        # the labelled rows and the table as the products read them, and the rows' places and
-        # statistics: kept for the backward
-        keep = h.new_empty(nhc + nec + nst)
-        ws = torch.empty(fwd, dtype=torch.float32, device=h.device)
-        loss = torch.empty(labels.shape if mode == 2 else (), dtype=torch.float32, device=h.device)
-        hc = keep.data_ptr()
-        ec, state = hc + 2 * nhc, hc + 2 * (nhc + nec)
-        _run(dev, "loss_fwd", lib.sg_loss_fwd, h.data_ptr(), table.data_ptr(), labels.data_ptr(),
-             int(labels.dtype == torch.int64), ignore, hc, ec, state, ws.data_ptr(), loss.data_ptr(), N, V, H, mode, fp16)
-        ctx.save_for_backward(keep)
-        ctx.plan = (lib.sg_loss_bwd, dev, shape, (N, V, H, mode, fp16), nhc, nec, bwd)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        (keep,) = ctx.saved_tensors
-        fn, dev, shape, dims, nhc, nec, words = ctx.plan
-        g = g.contiguous()
-        hc = keep.data_ptr()
-        dh = keep.new_empty(shape) if ctx.needs_input_grad[0] else None
-        dt = keep.new_empty(dims[1], dims[2]) if ctx.needs_input_grad[1] else None
-        ws = g.new_empty(words)
-        _run(dev, "loss_bwd", fn, hc, hc + 2 * nhc, hc + 2 * (nhc + nec), g.data_ptr(), ws.data_ptr(), ops._p(dh),
-             ops._p(dt), *dims)
-        return dh, dt, None, None, None
 
 
 def lm_loss(h: torch.Tensor, table: torch.Tensor, labels: torch.Tensor, *, reduction: str = "mean",
@@ -470,7 +318,7 @@ def lm_loss(h: torch.Tensor, table: torch.Tensor, labels: torch.Tensor, *, reduc
     if not -(1 << 31) <= ignore_index < 1 << 31:
         raise ValueError("lm_loss: ignore_index must fit 32 bits")
     _on_gpu("lm_loss", h, table, labels)
-    return _LmLoss.apply(h, table, labels, _REDUCTIONS[reduction], int(ignore_index))
+    return _native().loss(h, table, labels, _REDUCTIONS[reduction], int(ignore_index))
 
 
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:

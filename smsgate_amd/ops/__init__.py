@@ -14,6 +14,7 @@ references the numerics tests compare against.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from typing import Optional
 
@@ -24,6 +25,7 @@ from . import build as _build
 
 __all__ = [
     "load_library",
+    "load_train_autograd",
     "have_kernels",
     "rmsnorm_residual",
     "silu_mul",
@@ -61,6 +63,7 @@ __all__ = [
 ]
 
 _lib: Optional[ctypes.CDLL] = None
+_train_autograd = None
 _c_int = ctypes.c_int
 _c_float = ctypes.c_float
 _vp = ctypes.c_void_p
@@ -201,6 +204,21 @@ def load_library(build_if_missing: bool = True) -> ctypes.CDLL:
     _declare(lib)
     _lib = lib
     return lib
+
+
+def load_train_autograd():
+    """The training operators' autograd functions (csrc/train_autograd.cpp), an extension
+    module that calls the kernel library."""
+    global _train_autograd
+    if _train_autograd is None:
+        load_library()  # its entries, and built together
+        if _build.needs_build_autograd():
+            _build.build_autograd()
+        spec = importlib.util.spec_from_file_location(_build.AUTOGRAD.stem, _build.AUTOGRAD)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _train_autograd = mod
+    return _train_autograd
 
 
 def have_kernels() -> bool:

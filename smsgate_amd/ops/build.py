@@ -6,6 +6,11 @@ library exposes a plain C ABI and is loaded with ``ctypes`` — no torch C++
 headers (fast builds, no ABI coupling, no hipify step) — and every launch
 takes the caller's ``hipStream_t`` so it can be captured into a hipGraph.
 The build is skipped when the .so is newer than all sources.
+
+One part is built against torch's headers: ``csrc/train_autograd.cpp``, the training
+operators' autograd functions, into ``_lib/smsgate_train_autograd.so``.  A small training call
+is host time, and a Python Function costs more of it than all its kernels.  It links the
+kernel library, whose entries keep their C ABI.
 """
 from __future__ import annotations
 
@@ -13,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 from typing import List, Optional
 
@@ -20,6 +26,8 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIBDIR = HERE / "_lib"
 LIB = LIBDIR / "libsmsgate_kernels.so"
+AUTOGRAD_SRC = CSRC / "train_autograd.cpp"
+AUTOGRAD = LIBDIR / "smsgate_train_autograd.so"
 ARCH = os.environ.get("SMSGATE_OFFLOAD_ARCH", "gfx950")
 
 
@@ -78,6 +86,57 @@ def build(force: bool = False, verbose: bool = False, extra: Optional[List[str]]
     return LIB
 
 
+def needs_build_autograd() -> bool:
+    if not AUTOGRAD.exists():
+        return True
+    mt = AUTOGRAD.stat().st_mtime
+    return any(s.stat().st_mtime > mt for s in (AUTOGRAD_SRC, CSRC / "train_ops.hpp"))
+
+
+def build_autograd(force: bool = False, verbose: bool = False) -> Path:
+    """``csrc/train_autograd.cpp`` for this interpreter and torch; after :func:`build`, whose
+    library it links."""
+    if not force and not needs_build_autograd():
+        return AUTOGRAD
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    tmp = AUTOGRAD.with_suffix(".so.tmp")
+    cmd = [
+        os.environ.get("CXX", "g++"),
+        "-O2",
+        "-std=c++17",
+        "-fPIC",
+        "-shared",
+        "-D__HIP_PLATFORM_AMD__=1",  # torch's and HIP's headers on ROCm ask for both
+        "-DUSE_ROCM=1",
+        f"-DTORCH_EXTENSION_NAME={AUTOGRAD.stem}",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *(x for d in (root / "include", root / "include/torch/csrc/api/include",
+                      Path(hipcc()).resolve().parent.parent / "include", sysconfig.get_paths()["include"])
+          for x in ("-isystem", str(d))),
+        str(AUTOGRAD_SRC),
+        "-o",
+        str(tmp),
+        f"-L{root / 'lib'}",
+        "-ltorch",
+        "-ltorch_cpu",
+        "-ltorch_hip",
+        "-lc10",
+        "-lc10_hip",
+        "-ltorch_python",
+        f"-L{LIBDIR}",
+        f"-l:{LIB.name}",
+        "-Wl,-rpath,$ORIGIN",
+    ]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, AUTOGRAD)
+    return AUTOGRAD
+
+
 if __name__ == "__main__":
     p = build(force="--force" in sys.argv, verbose=True)
     print(p)
+    print(build_autograd(force="--force" in sys.argv, verbose=True))

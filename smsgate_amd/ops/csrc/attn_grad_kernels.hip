@@ -48,6 +48,8 @@
 #include <stdint.h>
 #include <type_traits>
 
+#include "train_ops.hpp"
+
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));

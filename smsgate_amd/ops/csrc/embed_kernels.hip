@@ -24,6 +24,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "train_ops.hpp"
+
 namespace {
 
 constexpr int EG_SMALL = 256;    // entries that the one-launch gradient takes

@@ -41,6 +41,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "train_ops.hpp"
+
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
