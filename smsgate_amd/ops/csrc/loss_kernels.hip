@@ -5,14 +5,14 @@
 //   d_i[v] = w_i (exp(z_i[v] - L_i) - [v = y_i]),  dh = f d E,  dE = f d^T h
 //
 // h [N, H] and E [V, H] in bf16 or fp16, H a multiple of 8, any N and V.  Rows whose label
-// is ignore_index are left out before any product: loss_rows lists the others, loss_layout
+// is ignore_index are left out before any product: loss_rows lists the others, loss_hidden
 // copies them together, and every later block reads the count from the device and ends at
 // once behind it (an SMS batch labels about a third of its positions).
 //
 //   forward   loss_logits<0>: a tile's logits stay in the accumulators; each row's maximum
 //             and sum of exponentials over the tile go out (8 bytes a row and tile), the label's
 //             logit from the tile that has it;
-//             loss_join: L and loss
+//             loss_join: L, loss and its mean or sum
 //   backward  per piece of the vocabulary: loss_logits<1> recomputes the tile's logits and
 //             writes d in the inputs' type; loss_grad: the piece's rows of dE, and dh's
 //             shares, fp32, the piece's columns split over blocks; loss_dh sums the shares in
@@ -27,7 +27,7 @@
 //
 // Products: v_mfma_f32_32x32x16, result in lane l: column l & 31 (the "lane" side: a hidden
 // row, or a vocabulary row for dE), rows (r & 3) + 8 (r >> 2) + 4 (l >> 5) (the "register"
-// side).  h, E and d lie in panels of 32 columns (loss_layout copies h's rows and E once a
+// side).  h, E and d lie in panels of 32 columns (h's rows and E are copied once a
 // call); a tile comes by DMA (global_load_lds) into two buffers, one barrier a 32-wide step.
 // Operands whose k runs along a panel's rows are read from LDS as rows, others by transposing
 // reads (ds_read_b64_tr_b16), so no transposed copy exists.
@@ -62,8 +62,8 @@ struct LossArgs {
   const uint16_t *h, *table;
   const void* labels;
   uint16_t *hc, *ec, *d, *dh, *dtable;  // hc, ec, d: panels
-  int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; [1]
-  float *lse, *rl, *loss, *w;       // [Mp] L; [Mp] label's logit, then loss; out; [Mp] row weights or null
+  int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; rows, blocks done
+  float *lse, *rl, *loss, *w;       // [Mp] L; [Mp] label's logit; out; [Mp] row weights or null
   float2* part;                     // [v tiles][Mp] (maximum, sum of exp(z - maximum))
   float* share;                     // [splits][Mp][Hp]
   const float *g, *gmax;            // incoming gradient; none: its largest magnitude
@@ -135,56 +135,7 @@ __device__ __forceinline__ float4 lk_four(const f32x16& x, int e, float f) {
   return make_float4(x[4 * e] * f, x[4 * e + 1] * f, x[4 * e + 2] * f, x[4 * e + 3] * f);
 }
 
-// ---- rows with a label -----------------------------------------------------------------
-// One block: places of the labelled rows, in order.  A label outside [0, V) becomes -2 (its
-// loss and gradients are NaN).
-__global__ void __launch_bounds__(1024) loss_rows_kernel(LossArgs a) {
-  __shared__ int part[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const unsigned long long before = (1ull << lane) - 1;
-  int base = 0;
-  for (int i0 = 0; i0 < a.N; i0 += 16384) {  // a wave owns 1024 labels, 64 at a time
-    const int w0 = i0 + 1024 * wave + lane;
-    long y[16];
-    int n = 0;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int i = w0 + 64 * k;
-      y[k] = i < a.N ? (a.is64 ? reinterpret_cast<const long*>(a.labels)[i]
-                               : (long)reinterpret_cast<const int*>(a.labels)[i])
-                     : a.ignore;
-    }
-#pragma unroll
-    for (int k = 0; k < 16; ++k) n += __popcll(__ballot(y[k] != a.ignore));
-    if (lane == 0) part[wave] = n;
-    __syncthreads();
-    int at = base, all = 0;
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) at += part[w];
-      all += part[w];
-    }
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int i = w0 + 64 * k;
-      const bool on = y[k] != a.ignore;
-      const unsigned long long m = __ballot(on);
-      const int place = at + __popcll(m & before);
-      at += __popcll(m);
-      if (i >= a.N) continue;
-      a.pos[i] = on ? place : -1;
-      if (on) {
-        a.rows[place] = i;
-        a.lab[place] = y[k] >= 0 && y[k] < a.V ? (int)y[k] : -2;
-      } else if (a.mode == 2) {
-        a.loss[i] = 0.f;
-      }
-    }
-    base += all;
-    __syncthreads();
-  }
-  if (tid == 0) a.cnt[0] = base;
-}
-
+// ---- rows with a label, operands in panels ------------------------------------------------
 // Every operand of the products lies in panels of LK_PANEL columns, [panel][rows][LK_PANEL]:
 // a tile is runs of memory of 1 KB and more whichever way it is read, nothing of it is out of
 // bounds, and its copies need no address but a wave's own.  (Tiles of the matrices as they
@@ -194,23 +145,106 @@ __device__ __forceinline__ size_t lk_at(long rows, long row, int c) {  // 16-byt
   return ((c >> 2) * rows + row) * LK_PANEL + (c & 3) * 8;
 }
 
-// hc = h[rows] (zeros behind the last row, up to a whole tile, and column) and ec = E, in
-// panels; 16 bytes a thread
-__global__ void __launch_bounds__(256) loss_layout_kernel(LossArgs a) {
-  const int nch = a.Hp / 8, cnt = a.cnt[0];
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+// 16-byte chunk i of ec = E in panels, zeros behind its rows and columns
+__device__ __forceinline__ void lk_lay_table(const LossArgs& a, long i) {
+  const int nch = a.Hp / 8;
   const long r = i / nch;
   const int c = (int)(i - r * nch);
+  if (r >= a.Vp) return;
   uint4 v = make_uint4(0, 0, 0, 0);
-  if (r < a.Vp) {
-    if (r < a.V && 8 * c < a.H) v = *reinterpret_cast<const uint4*>(a.table + (size_t)r * a.H + 8 * c);
-    *reinterpret_cast<uint4*>(a.ec + lk_at(a.Vp, r, c)) = v;
+  if (r < a.V && 8 * c < a.H) v = *reinterpret_cast<const uint4*>(a.table + (size_t)r * a.H + 8 * c);
+  *reinterpret_cast<uint4*>(a.ec + lk_at(a.Vp, r, c)) = v;
+}
+
+// ... of hc = h[rows], zeros behind the last row up to a whole tile
+__device__ __forceinline__ void lk_lay_hidden(const LossArgs& a, long i, int cnt, const int* rows) {
+  const int nch = a.Hp / 8, m = (int)(i / nch), c = (int)(i - (long)m * nch);
+  if (m >= (cnt + LK_PAD - 1) / LK_PAD * LK_PAD || m >= a.Mp) return;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (m < cnt && 8 * c < a.H) v = *reinterpret_cast<const uint4*>(a.h + (size_t)rows[m] * a.H + 8 * c);
+  *reinterpret_cast<uint4*>(a.hc + lk_at(a.Mp, m, c)) = v;
+}
+
+__device__ __forceinline__ long lk_label(const LossArgs& a, int i) {
+  return i >= a.N     ? a.ignore
+         : a.is64 ? reinterpret_cast<const long*>(a.labels)[i]
+                  : (long)reinterpret_cast<const int*>(a.labels)[i];
+}
+
+// What is known of row i: its place (or none).  A label outside [0, V) becomes -2 (its loss
+// and gradients are NaN).
+__device__ __forceinline__ void lk_put(const LossArgs& a, int i, long y, int place) {
+  if (i >= a.N) return;
+  const bool on = y != a.ignore;
+  a.pos[i] = on ? place : -1;
+  if (on) {
+    a.rows[place] = i;
+    a.lab[place] = y >= 0 && y < a.V ? (int)y : -2;
+  } else if (a.mode == 2) {
+    a.loss[i] = 0.f;
+  }
+}
+
+constexpr int LK_SMALL = 1024;  // rows that a block numbers by itself
+
+// The table in panels (the blocks from nb on), and the places of the labelled rows, in order.
+// SMALL (up to LK_SMALL rows): every hidden block numbers the rows by itself and copies its
+// part of them, so that one launch does all; else block 0 numbers them beside the table's
+// copy, and loss_hidden follows.
+template <bool SMALL>
+__global__ void __launch_bounds__(1024) loss_rows_kernel(LossArgs a, int nb) {
+  __shared__ int part[16], list[SMALL ? LK_SMALL : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if ((int)blockIdx.x >= nb) {
+    lk_lay_table(a, (long)(blockIdx.x - nb) * 1024 + tid);
     return;
   }
-  const int m = (int)(r - a.Vp);
-  if (m >= (cnt + LK_PAD - 1) / LK_PAD * LK_PAD || m >= a.Mp) return;
-  if (m < cnt && 8 * c < a.H) v = *reinterpret_cast<const uint4*>(a.h + (size_t)a.rows[m] * a.H + 8 * c);
-  *reinterpret_cast<uint4*>(a.hc + lk_at(a.Mp, m, c)) = v;
+  const unsigned long long before = (1ull << lane) - 1;
+  int cnt = 0;
+  if constexpr (SMALL) {
+    const long y = lk_label(a, tid);
+    const unsigned long long m = __ballot(y != a.ignore);
+    if (lane == 0) part[wave] = __popcll(m);
+    __syncthreads();
+    int at = __popcll(m & before);
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) at += part[w];
+      cnt += part[w];
+    }
+    if (y != a.ignore) list[at] = tid;
+    if (blockIdx.x == 0) lk_put(a, tid, y, at);
+    __syncthreads();
+    lk_lay_hidden(a, (long)blockIdx.x * 1024 + tid, cnt, list);
+  } else {
+    for (int i0 = 0; i0 < a.N; i0 += 16384) {  // a wave owns 1024 labels, 64 at a time
+      const int w0 = i0 + 1024 * wave + lane;
+      long y[16];
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) y[k] = lk_label(a, w0 + 64 * k);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) n += __popcll(__ballot(y[k] != a.ignore));
+      if (lane == 0) part[wave] = n;
+      __syncthreads();
+      int at = cnt;
+      for (int w = 0; w < 16; ++w) {
+        if (w < wave) at += part[w];
+        cnt += part[w];
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const unsigned long long m = __ballot(y[k] != a.ignore);
+        lk_put(a, w0 + 64 * k, y[k], at + __popcll(m & before));
+        at += __popcll(m);
+      }
+      __syncthreads();
+    }
+  }
+  if (blockIdx.x == 0 && tid == 0) a.cnt[0] = cnt, a.cnt[1] = 0;
+}
+
+__global__ void __launch_bounds__(256) loss_hidden_kernel(LossArgs a) {
+  lk_lay_hidden(a, (long)blockIdx.x * 256 + threadIdx.x, a.cnt[0], a.rows);
 }
 
 // ---- products --------------------------------------------------------------------------
@@ -502,11 +536,48 @@ __global__ void __launch_bounds__(WL * WR * 64, 3) loss_grad_kernel(LossArgs a) 
 }
 
 // ---- joins -----------------------------------------------------------------------------
-// 16 rows a block: L from the tiles' (maximum, sum), the label's logit, the loss.
+// The loss from the join's sums (of block b over its own rows' first tile in part, 32 b), in
+// their order; mean: no labelled row gives 0 / 0, as the mean of nothing.  One block of 256.
+__device__ __forceinline__ void lk_total(const LossArgs& a, int blocks, float* red) {
+  const float* sums = reinterpret_cast<const float*>(a.part);
+  float s = 0.f;
+  for (int b0 = threadIdx.x; b0 < blocks; b0 += 1024) {
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] = 0.f;
+      if (b0 + 256 * k < blocks)
+        x[k] = __hip_atomic_load(sums + 32 * (size_t)(b0 + 256 * k), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    s += (x[0] + x[1]) + (x[2] + x[3]);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = (red[0] + red[1]) + (red[2] + red[3]);
+    a.loss[0] = a.mode == 0 ? s / (float)a.cnt[0] : s;
+  }
+}
+
+__device__ __forceinline__ int lk_join_blocks(int cnt) { return max(1, (cnt + 15) / 16); }
+
+__global__ void __launch_bounds__(256) loss_sum_kernel(LossArgs a) {
+  __shared__ float red[4];
+  lk_total(a, lk_join_blocks(a.cnt[0]), red);
+}
+
+// 16 rows a block: L from the tiles' (maximum, sum), the label's logit, the loss.  TOTAL: the
+// block that ends last, whichever it is, takes the total too.  That saves a small call a
+// launch (5.0 us for 4.2 + 3.5), but every block's sum has to reach the others' caches: 300
+// blocks take 14.1 us with it for 4.4 + 4.3.
+template <bool TOTAL>
 __global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
   __shared__ float2 red[16][16];
-  const int m0 = blockIdx.x * 16, cnt = a.cnt[0];
-  if (m0 >= cnt) return;
+  __shared__ bool last;
+  const int m0 = blockIdx.x * 16, cnt = a.cnt[0], blocks = lk_join_blocks(cnt);
+  if ((int)blockIdx.x >= blocks) return;
   const int r = threadIdx.x & 15, g = threadIdx.x >> 4;  // row, share of the tiles
   float2 x = make_float2(-INFINITY, 0.f);
   for (int t = g; t < tiles; t += 64) {
@@ -528,41 +599,34 @@ __global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
   red[g][r] = x;
   __syncthreads();
   const int m = m0 + threadIdx.x;
-  if (threadIdx.x >= 16 || m >= cnt) return;
-  float top = -INFINITY;
+  float loss = 0.f;
+  if (threadIdx.x < 16 && m < cnt) {
+    float top = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) top = fmaxf(top, red[w][threadIdx.x].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float s = 0.f;
+    for (int w = 0; w < 16; ++w) top = fmaxf(top, red[w][threadIdx.x].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float s = 0.f;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) s += red[w][threadIdx.x].y * lk_exp_fine(red[w][threadIdx.x].x - ref);
-  float ls = logf(s);  // (not the hardware's log2: near 1 it is off by more than an ulp)
-  if (a.lab[m] == -2) ls = __builtin_nanf("");
-  const float loss = (top - a.rl[m]) + ls;
-  a.lse[m] = top + ls;
-  a.rl[m] = loss;
-  if (a.mode == 2) a.loss[a.rows[m]] = loss;
-}
-
-__device__ __forceinline__ float lk_block_sum(float s, float* red) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int w = 0; w < 16; ++w) s += red[w][threadIdx.x].y * lk_exp_fine(red[w][threadIdx.x].x - ref);
+    float ls = logf(s);  // (not the hardware's log2: near 1 it is off by more than an ulp)
+    if (a.lab[m] == -2) ls = __builtin_nanf("");
+    loss = (top - a.rl[m]) + ls;
+    a.lse[m] = top + ls;
+    if (a.mode == 2) a.loss[a.rows[m]] = loss;
+  }
+  if (a.mode == 2) return;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if (lane == 0) red[wave] = s;
-  __syncthreads();
-  s = 0.f;
-  for (int w = 0; w < 16; ++w) s += red[w];
-  return s;
-}
-
-// mean (no labelled row: 0 / 0, as the mean of nothing) or sum
-__global__ void __launch_bounds__(1024) loss_sum_kernel(LossArgs a) {
-  __shared__ float red[16];
-  const int cnt = a.cnt[0];
-  float s = 0.f;
-  for (int m = threadIdx.x; m < cnt; m += 1024) s += a.rl[m];
-  s = lk_block_sum(s, red);
-  if (threadIdx.x == 0) a.loss[0] = a.mode == 0 ? s / (float)cnt : s;
+  for (int o = 8; o > 0; o >>= 1) loss += __shfl_xor(loss, o, 64);
+  if (threadIdx.x == 0) reinterpret_cast<float*>(a.part)[2 * (size_t)m0] = loss;
+  if constexpr (TOTAL) {
+    if (threadIdx.x == 0) {
+      __threadfence();
+      last = atomicAdd(&a.cnt[1], 1) == blocks - 1;
+      __threadfence();
+    }
+    __syncthreads();
+    if (last) lk_total(a, blocks, reinterpret_cast<float*>(red));
+  }
 }
 
 // none: gmax = the largest finite |g|, w = g / gmax (in [-1, 1])
@@ -671,13 +735,22 @@ void lk_grads(LossArgs a, const LossPlan& p, hipStream_t st) {
 
 template <bool BF>
 void lk_forward(LossArgs a, const LossPlan& p, hipStream_t st) {
-  loss_rows_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
-  loss_layout_kernel<<<dim3((unsigned)(((long)(p.Mp + a.Vp) * (p.Hp / 8) + 255) / 256)), dim3(256), 0, st>>>(a);
+  const long nch = p.Hp / 8, hidden = (p.Mp * nch + 1023) / 1024, table = (a.Vp * nch + 1023) / 1024;
+  if (a.N <= LK_SMALL) {
+    loss_rows_kernel<true><<<dim3((unsigned)(hidden + table)), dim3(1024), 0, st>>>(a, (int)hidden);
+  } else {
+    loss_rows_kernel<false><<<dim3((unsigned)(1 + table)), dim3(1024), 0, st>>>(a, 1);
+    loss_hidden_kernel<<<dim3((unsigned)((p.Mp * nch + 255) / 256)), dim3(256), 0, st>>>(a);
+  }
   a.v0 = 0;
   a.vn = p.vtiles * (p.small ? 64 : 256);
   lk_logits<BF, 0>(a, p, st);
-  loss_join_kernel<<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
-  if (a.mode != 2) loss_sum_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
+  if (a.N <= LK_SMALL && a.mode != 2) {
+    loss_join_kernel<true><<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
+    return;
+  }
+  loss_join_kernel<false><<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
+  if (a.mode != 2) loss_sum_kernel<<<dim3(1), dim3(256), 0, st>>>(a);
 }
 
 template <bool BF>
