@@ -47,12 +47,9 @@ Tensor rows16(const Tensor& t) {
 Tensor words(const Tensor& like, int64_t n) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 
 // The gradients of a backward that can be run but not differentiated: under create_graph they
-// carry a function that raises.
-variable_list once(variable_list grads, variable_list out) {
-  if (!at::GradMode::is_enabled()) return out;
-  bool any = false;
-  for (const Tensor& g : grads) any = any || (g.defined() && g.requires_grad());
-  if (!any) return out;
+// carry a function that raises.  linear: they depend on the incoming gradient alone.
+variable_list once(const variable_list& grads, variable_list out, bool linear) {
+  if (!at::GradMode::is_enabled() || (linear && !grads[0].requires_grad())) return out;
   variable_list some;
   for (Tensor& t : out)
     if (t.defined()) some.push_back(t.requires_grad_());
@@ -108,7 +105,7 @@ struct Embed : torch::autograd::Function<Embed> {
         dt.zero_();
       }
     }
-    return once(grads, {dt, Tensor(), Tensor(), Tensor()});
+    return once(grads, {dt, Tensor(), Tensor(), Tensor()}, true);
   }
 };
 
@@ -163,7 +160,7 @@ struct Attention : torch::autograd::Function<Attention> {
           (const void*)lse, ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(ws), (const void*)s.strides, s.B, s.T, s.nh, s.nkv,
           s.D, (int)ctx->saved_data["causal"].toBool(), s.fp16, (float)ctx->saved_data["scale"].toDouble());
     }
-    return once(grads, {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()});
+    return once(grads, {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()}, false);
   }
 };
 
@@ -220,7 +217,7 @@ struct Loss : torch::autograd::Function<Loss> {
           ptr(ws), ptr(dh), ptr(dt), (int)N, (int)V, (int)H, (int)ctx->saved_data["mode"].toInt(),
           (int)(keep.scalar_type() == at::kHalf));
     }
-    return once(grads, {dh, dt, Tensor(), Tensor(), Tensor()});
+    return once(grads, {dh, dt, Tensor(), Tensor(), Tensor()}, false);
   }
 };
 
