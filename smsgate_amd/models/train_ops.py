@@ -36,7 +36,8 @@ and a Python Function spends 1.4 times as much of it (45 positions forward and b
 
 Their forward and backward can be captured into a graph.  As with any torch operator, no
 eager graph of the same leaves may be alive then: a leaf's accumulation node belongs to the
-stream that it was first used on, and autograd waits for that stream inside the capture.
+stream that it was first used on, and autograd would wait for that stream inside the capture.
+Where such a leaf is an operator's own input, the captured call raises.
 
 GEMMs stay hipBLASLt (autocast bf16), so the math is
 reference_forward's up to bf16 rounding order (tests/test_train_ops_gpu.py compares

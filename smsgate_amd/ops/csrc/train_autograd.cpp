@@ -221,7 +221,26 @@ struct Loss : torch::autograd::Function<Loss> {
   }
 };
 
+// Capturing a call whose leaf takes part in a living eager graph is refused: the leaf's
+// accumulation node belongs to that graph's stream, autograd would wait for it in the captured
+// backward, and the process would end.
+void no_eager_graph(std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  const auto st = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA((*inputs.begin())->device().index());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing(st.stream(), &status) == hipSuccess, "hipStreamIsCapturing failed");
+  if (status == hipStreamCaptureStatusNone) return;
+  for (const Tensor* t : inputs) {
+    if (!t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto of = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!of || *of == st.unwrap(),
+                "a captured call shares a leaf with a living eager graph: drop that graph's results first");
+  }
+}
+
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& lens, double scale, bool causal) {
+  no_eager_graph({&q, &k, &v});
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
   return Attention::apply(q, k, v, lens, scale, causal, grad);
 }
@@ -231,10 +250,12 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe&
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   const auto free = py::call_guard<py::gil_scoped_release>();
   m.def("embed", [](const Tensor& table, const Tensor& ids, const Maybe& add, double scale) {
+    no_eager_graph({&table});
     return Embed::apply(table, ids, add, scale);
   }, free);
   m.def("attention", &attention, free);
   m.def("loss", [](const Tensor& h, const Tensor& table, const Tensor& labels, int64_t mode, int64_t ignore) {
+    no_eager_graph({&h, &table});
     return Loss::apply(h, table, labels, mode, ignore);
   }, free);
   m.def("rows16", &rows16);

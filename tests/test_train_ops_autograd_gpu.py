@@ -108,3 +108,25 @@ def test_memory_goes_with_the_results():
             if _ == 0:
                 first = held
         assert held == first, name
+
+
+def test_capture_beside_a_living_eager_graph_is_refused():
+    """The captured backward would end the process; the captured forward raises instead."""
+    for name, leaves, call in _calls():
+        alive = call(*leaves)
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(graph):
+                call(*leaves)
+        want = torch.autograd.grad(alive, leaves, torch.ones_like(alive))
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(*leaves)
+            got = torch.autograd.grad(out, leaves, torch.ones_like(out))
+            del out
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, w in zip(got, want):
+                assert torch.equal(x, w), name
