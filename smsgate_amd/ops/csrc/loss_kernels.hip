@@ -36,7 +36,7 @@
 // less time with the copies left out, none with LDS reads or exp left out), and that a block's
 // waves wait together: three blocks a CU of 128 x 256 (165 registers) beat two of them with
 // deeper buffers (467 us against 491) and one of 256 x 256 (518).  Measured at 8192 rows, 49152
-// ids, 576 columns, bf16: logits 467 us (993 TFLOP/s), d 525, both gradients 1097 (846
+// ids, 576 columns, bf16: logits 467 us (993 TFLOP/s), d 525, both gradients 1057 (878
 // TFLOP/s); the library's single products of these shapes take 539, 604 and 750.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -62,7 +62,7 @@ struct LossArgs {
   const uint16_t *h, *table;
   const void* labels;
   uint16_t *hc, *ec, *d, *dh, *dtable;  // hc, ec, d: panels
-  int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; rows, blocks done
+  int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; rows, blocks done, splits
   float *lse, *rl, *loss, *w;       // [Mp] L; [Mp] label's logit; out; [Mp] row weights or null
   float2* part;                     // [v tiles][Mp] (maximum, sum of exp(z - maximum))
   float* share;                     // [splits][Mp][Hp]
@@ -70,7 +70,7 @@ struct LossArgs {
   long ignore;
   int N, V, H, Mp, Hp, Vp, is64, mode;  // mode 0 mean, 1 sum, 2 none
   int v0, vn;                       // piece: first row, rows (of them < V - v0 real)
-  int splits, want, most, first;    // dh: shares of Mp rows in the workspace; blocks wanted; splits at most
+  int splits, want, most, first;    // dh: shares of Mp rows in the workspace; the card's places; splits at most
   int bl, nr;                       // dh: rows of a tile, tiles over H
   int t2;                           // blocks of dE, a multiple of 8
 };
@@ -288,13 +288,43 @@ __device__ __forceinline__ void lk_stage(const uint16_t* src, long stride, int p
   }
 }
 
-// Splits of the piece's columns that dh's share is taken in, for `tiles` tiles over `rows`
-// rows: enough blocks for the card, as many as the workspace holds.  The same for every
-// piece, so that later pieces add to the shares of the first.
-__device__ __forceinline__ int lk_splits(int rows, int tiles, const LossArgs& a) {
-  if (rows == 0) return 1;
-  const int fit = (int)((long)a.splits * a.Mp / rows), want = (a.want + tiles - 1) / tiles;
-  return max(1, min(min(fit, want), a.most));
+// Splits of the piece's columns that dh's shares are taken in (the same for every piece, so
+// that later pieces add to the shares of the first), chosen once for the count of rows by the
+// 64 lanes of a wave, one candidate each: the end of the launch if its blocks go to the card's
+// places in turn, dE's first, and the shares' memory time.  Steps of the blocks that end last
+// count 0.73 us each (a block among others; with all places full a step's work adds 0.68 us
+// whatever the split), a share's float 1.7e-6 us, written and read; over 1 to 11 splits of the
+// three large cases the sum is within 8 % of what was measured, but for launches that leave
+// most places empty.  (8192 rows, 16384 of the ids, 576 columns: 2 splits 362 us, 3 432, 4 376,
+// 5 433; a fixed number of blocks picked 4.)
+__device__ int lk_choose(const LossArgs& a, int cnt, int lane) {
+  const int nl = (cnt + a.bl - 1) / a.bl, nh = nl * a.nr, s = lane + 1;
+  if (nh == 0) return 1;
+  const int fit = min(a.most, (int)((long)a.splits * a.Mp / ((long)nl * a.bl)));
+  const int ne = a.vn / a.bl * a.nr, e = (cnt + 31) / 32 + 4, r = ne % a.want;  // 4: a block's start and end
+  const int l = ((a.vn / LK_K + s - 1) / s * LK_K) / 32 + 4;
+  const float t0 = (float)(ne / a.want) * e, b = (float)nh * s;
+  // after t0 steps: want - r places free, r more e steps later
+  auto done = [&](float t) { return (a.want - r) * floorf(t / l) + r * floorf(fmaxf(t - e, 0.f) / l); };
+  const float x = (b * l + (float)r * e) / a.want;  // were blocks divisible
+  float end = INFINITY;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float p = (ceilf(x / l) + k) * l, q = e + (ceilf(fmaxf(x - e, 0.f) / l) + k) * l;
+    if (done(p) >= b) end = fminf(end, p);
+    if (done(q) >= b) end = fminf(end, q);
+  }
+  if (end == INFINITY) end = x + l;
+  end = t0 + fmaxf(end, r ? (float)e : 0.f);
+  float cost = s <= max(fit, 1) ? 0.73f * end + 1.7e-6f * s * cnt * a.Hp : INFINITY;
+  int best = s;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const float c = __shfl_xor(cost, o, 64);
+    const int n = __shfl_xor(best, o, 64);
+    if (c < cost || (c == cost && n < best)) cost = c, best = n;
+  }
+  return best;
 }
 
 // MODE 0 / 1: lane side = hidden rows, register side = vocabulary rows, k = H.
@@ -318,7 +348,7 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
   const int cnt = a.cnt[0];
   const int nl = MODE == 2 ? a.vn / BL : (cnt + BL - 1) / BL;
   const int nr = MODE >= 2 ? (a.H + BR - 1) / BR : a.vn / BR;
-  const int splits = MODE == 3 ? lk_splits(nl * BL, nl * nr, a) : 1;
+  const int splits = MODE == 3 ? a.cnt[2] : 1;
   // blocks go round the 8 XCDs: each gets a run of tiles, walked in bands of 8 lane-side
   // tiles, so that what an XCD has in flight shares its L2.  Runs of the labelled rows'
   // tiles only (the grid holds all rows'): else a few XCDs would have all the work
@@ -577,6 +607,12 @@ __global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
   __shared__ float2 red[16][16];
   __shared__ bool last;
   const int m0 = blockIdx.x * 16, cnt = a.cnt[0], blocks = lk_join_blocks(cnt);
+  if (blockIdx.x == gridDim.x - 1) {  // a block more: the backward's splits
+    if (threadIdx.x >= 64) return;
+    const int splits = lk_choose(a, cnt, threadIdx.x);
+    if (threadIdx.x == 0) a.cnt[2] = splits;
+    return;
+  }
   if ((int)blockIdx.x >= blocks) return;
   const int r = threadIdx.x & 15, g = threadIdx.x >> 4;  // row, share of the tiles
   float2 x = make_float2(-INFINITY, 0.f);
@@ -660,7 +696,7 @@ __global__ void __launch_bounds__(256) loss_dh_kernel(LossArgs a) {
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (m >= 0) {
     const int rows = (a.cnt[0] + a.bl - 1) / a.bl * a.bl;
-    const int splits = lk_splits(rows, rows / a.bl * a.nr, a);
+    const int splits = a.cnt[2];
     for (int z0 = 0; z0 < splits; z0 += 8) {
       float4 x[8];
 #pragma unroll
@@ -715,15 +751,14 @@ void lk_logits(const LossArgs& a, const LossPlan& p, hipStream_t st) {
     loss_logits_kernel<BF, MODE, 128, 256, 1, 4, 2><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
 }
 
-// dh has as many blocks as any count of rows may want (lk_splits: tiles x splits is at most
-// tiles + want, and at most the workspace's shares).
+// dh has as many blocks as any count of rows may want (its tiles' rows x splits are at most the
+// workspace's shares).
 template <bool BF>
 void lk_grads(LossArgs a, const LossPlan& p, hipStream_t st) {
   a.t2 = a.dtable != nullptr ? (a.vn / a.bl * a.nr + 7) / 8 * 8 : 0;
   long t3 = 0;
   if (a.dh != nullptr) {
-    const long nl = a.Mp / a.bl, all = nl * a.nr * a.splits, some = nl * a.nr + a.want;
-    t3 = all < some ? all : some;
+    t3 = (long)a.Mp / a.bl * a.nr * a.splits;
   }
   if (a.t2 + t3 == 0) return;
   const dim3 grid((unsigned)(a.t2 + t3));
@@ -745,19 +780,18 @@ void lk_forward(LossArgs a, const LossPlan& p, hipStream_t st) {
   a.v0 = 0;
   a.vn = p.vtiles * (p.small ? 64 : 256);
   lk_logits<BF, 0>(a, p, st);
+  a.vn = a.vn < p.piece ? a.vn : p.piece;  // (for the choice of the backward's splits)
   if (a.N <= LK_SMALL && a.mode != 2) {
-    loss_join_kernel<true><<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
+    loss_join_kernel<true><<<dim3(p.Mp / 16 + 1), dim3(256), 0, st>>>(a, p.vtiles);
     return;
   }
-  loss_join_kernel<false><<<dim3(p.Mp / 16), dim3(256), 0, st>>>(a, p.vtiles);
+  loss_join_kernel<false><<<dim3(p.Mp / 16 + 1), dim3(256), 0, st>>>(a, p.vtiles);
   if (a.mode != 2) loss_sum_kernel<<<dim3(1), dim3(256), 0, st>>>(a);
 }
 
 template <bool BF>
 void lk_backward(LossArgs a, const LossPlan& p, hipStream_t st) {
   if (a.mode == 2) loss_weights_kernel<<<dim3(1), dim3(1024), 0, st>>>(a, const_cast<float*>(a.gmax));
-  a.splits = p.splits, a.want = p.want, a.most = p.most;
-  a.bl = p.small ? 64 : LK_BL, a.nr = p.small ? (a.H + 63) / 64 : (a.H + 191) / 192;
   const int vp = p.vtiles * (p.small ? 64 : 256);
   for (int v0 = 0; v0 < vp; v0 += p.piece) {
     a.v0 = v0;
@@ -786,6 +820,8 @@ void lk_state(LossArgs& a, const LossPlan& p, void* state) {
   a.rl = a.lse + p.Mp;
   a.pos = (int*)(a.rl + p.Mp);
   a.Mp = p.Mp, a.Hp = p.Hp, a.Vp = p.vtiles * (p.small ? 64 : 256);
+  a.splits = p.splits, a.want = p.want, a.most = p.most;
+  a.bl = p.small ? 64 : LK_BL, a.nr = p.small ? (a.H + 63) / 64 : (a.H + 191) / 192;
 }
 
 }  // namespace
