@@ -31,8 +31,8 @@ Three operators of the whole step, on request (``hip_ops``; TrainConfig.hip_ops)
   span answer formats (csrc/loss_kernels.hip).
 
 Their autograd functions are C++ (csrc/train_autograd.cpp): one message's call is host time,
-and a Python Function spends 1.4 times as much of it (45 positions forward and backward 37 ->
-27 us, attention of 37 rows 59 -> 42, the loss of 61 rows 70 -> 57).
+and a Python Function spends 1.3 times as much of it (45 positions forward and backward 36 ->
+26 us, attention of 37 rows 57 -> 40, the loss of 61 rows 60 -> 47).
 
 Their forward and backward can be captured into a graph.  As with any torch operator, no
 eager graph of the same leaves may be alive then: a leaf's accumulation node belongs to the

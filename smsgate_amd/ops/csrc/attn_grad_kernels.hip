@@ -33,9 +33,10 @@
 // Sums, L, D and the running maximum are fp32.  The forward keeps what rounding took from o
 // (another value of the type), so that D is taken from 16 more bits of o: from the rounded o
 // alone its error was a third of dq's and dk's (2.8e-3 instead of 2.3e-3 of their norm at
-// 61 rows, bf16).  P and dS are rounded to the inputs' type as
-// operands (at most 2^-8 relative in bf16, as the inputs themselves are; see at_mma_p).  fp16 holds no value under
-// 2^-24: there P is scaled by 2^8 and dS by a power of two that the longest rows of do and v set.
+// 61 rows, bf16).  P and dS are rounded to the inputs' type as operands (at most 2^-8 relative
+// in bf16, as the inputs themselves are; see at_mma_p).  fp16 holds no value under 2^-24: there
+// P is scaled by 2^8 (by 2^7 forward) and dS by a power of two that the longest rows of do and
+// v set.
 //
 // What bounds it: the waves' own chains (product, exp2, rounding, product): at 16384 rows the
 // matrix units work a third of the time, the vector units half, and neither copies (10 % less
@@ -43,7 +44,8 @@
 // hold it up.  4 waves a block: 2 took 404 -> 525 us forward, 700 -> 770 in attn_dkv (copies
 // are shared by fewer), 8 took 436 and 726 (one barrier holds more).  Measured, bf16, causal,
 // 9 / 3 heads of 64, 16384 rows: forward 404 us (766 TFLOP/s of the products that the mask
-// leaves), attn_dq 500, attn_dkv 700 (S and dP are each taken twice); 128 sequences of up to 61 rows: 15 + 15 + 12 us, 48 MB.
+// leaves), attn_dq 500, attn_dkv 700 (S and dP are each taken twice); 128 sequences of up to 61
+// rows: 15 + 16 + 12 us, 48 MB.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <type_traits>
