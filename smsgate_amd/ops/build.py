@@ -29,6 +29,26 @@ LIB = LIBDIR / "libsmsgate_kernels.so"
 AUTOGRAD_SRC = CSRC / "train_autograd.cpp"
 AUTOGRAD = LIBDIR / "smsgate_train_autograd.so"
 ARCH = os.environ.get("SMSGATE_OFFLOAD_ARCH", "gfx950")
+# what every HIP source is compiled with
+FLAGS = [
+    f"--offload-arch={ARCH}",
+    "-O3",
+    "-std=c++17",
+    "-fPIC",
+    "-munsafe-fp-atomics",
+    # MFMA accumulators in VGPRs: the default AGPR form made the GEMM K-loop
+    # shuffle its accumulators (68 v_accvgpr_* per 32 MFMAs) and cost the
+    # attention kernels one wave of occupancy (scripts/kernel_resources.py)
+    "-mllvm",
+    "-amdgpu-mfma-vgpr-form=1",
+    # no packed-fp32 instructions (v_pk_fma_f32 and its like, which -O3 forms from
+    # ordinary float code): some of their forms have given wrong results now and then.
+    # The host pass does not know the feature and says so; that warning is harmless
+    "-Xclang",
+    "-target-feature",
+    "-Xclang",
+    "-packed-fp32-ops",
+]
 
 
 def hipcc() -> str:
@@ -56,24 +76,8 @@ def build(force: bool = False, verbose: bool = False, extra: Optional[List[str]]
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [
         hipcc(),
-        f"--offload-arch={ARCH}",
-        "-O3",
-        "-std=c++17",
-        "-fPIC",
+        *FLAGS,
         "-shared",
-        "-munsafe-fp-atomics",
-        # MFMA accumulators in VGPRs: the default AGPR form made the GEMM K-loop
-        # shuffle its accumulators (68 v_accvgpr_* per 32 MFMAs) and cost the
-        # attention kernels one wave of occupancy (scripts/kernel_resources.py)
-        "-mllvm",
-        "-amdgpu-mfma-vgpr-form=1",
-        # no packed-fp32 instructions (v_pk_fma_f32 and its like, which -O3 forms from
-        # ordinary float code): some of their forms have given wrong results now and then.
-        # The host pass does not know the feature and says so; that warning is harmless
-        "-Xclang",
-        "-target-feature",
-        "-Xclang",
-        "-packed-fp32-ops",
         *(extra or []),
         *[str(s) for s in sources()],
         "-o",

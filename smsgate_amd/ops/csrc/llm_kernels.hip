@@ -1559,8 +1559,9 @@ __global__ void __launch_bounds__(64, MINW) attn_grouped_kernel(
 // ---------------------------------------------------------------------------
 // NCB column blocks of 16 (NCB = 2: up to 32 / G pseudo-rows, e.g. 1 + 8 drafts at
 // G = 3) share every K/V tile load; block cb holds columns 16·cb .. 16·cb + 15.
+// Two blocks (the engine's form) take 127 registers of the 128 that leave four waves a SIMD.
 template <int NCB>
-__global__ void __launch_bounds__(64) attn_spec_kernel(
+__global__ void __launch_bounds__(64, NCB == 2 ? 4 : 1) attn_spec_kernel(
     const uint16_t* __restrict__ q, const int* __restrict__ row_start, const int* __restrict__ row_nd,
     const int* __restrict__ x_pos, const int* __restrict__ x_slot, const int* __restrict__ x_done,
     const uint16_t* __restrict__ k_cache, const uint16_t* __restrict__ vt_cache, const uint16_t* __restrict__ pk,
@@ -1579,19 +1580,20 @@ __global__ void __launch_bounds__(64) attn_spec_kernel(
   float m[NCB], lsum[NCB];
   int own[NCB];
   bool col_valid[NCB];
-  size_t qrow[NCB];
+  uint32_t qrow[NCB];  // rows of q and out (of 128 bytes: fewer than 2^32 fit the card)
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
     const int c = 16 * cb + r16, i = c / G, g = c % G;
     col_valid[cb] = i < nq;
     own[cb] = p + i + 1;  // per-lane length (invalid columns: masked by q = 0 and no store)
-    qrow[cb] = (size_t)(st + (col_valid[cb] ? i : 0)) * nh + kh * G + g;
+    qrow[cb] = (uint32_t)(st + (col_valid[cb] ? i : 0)) * nh + kh * G + g;
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
-      uint4 v = *reinterpret_cast<const uint4*>(q + qrow[cb] * D + 8 * g4 + 32 * s2);
+      uint4 v = *reinterpret_cast<const uint4*>(q + (size_t)qrow[cb] * D + 8 * g4 + 32 * s2);
       if (!col_valid[cb]) v = make_uint4(0, 0, 0, 0);
       qb[cb][s2] = __builtin_bit_cast(bf16x8, v);
     }
+    asm("" : "+v"(qrow[cb]));  // kept as 32 bits: not the two registers of the row's address
 #pragma unroll
     for (int n = 0; n < 4; ++n) o[cb][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     m[cb] = -INFINITY;
@@ -1637,7 +1639,7 @@ __global__ void __launch_bounds__(64) attn_spec_kernel(
   for (int cb = 0; cb < NCB; ++cb) {
     if (!col_valid[cb]) continue;
     const float inv = 1.f / lsum[cb];
-    uint16_t* orow = out + qrow[cb] * D;
+    uint16_t* orow = out + (size_t)qrow[cb] * D;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       uint2 w;
@@ -1663,8 +1665,10 @@ __global__ void __launch_bounds__(64) attn_spec_kernel(
 // grid = (ceil(max_q / QPW), nseq, nkv), one wave.  PF = 1 (merged stream only): the
 // loads of key tile t+1 are issued before the MFMAs of tile t (one-tile register prefetch).
 // ---------------------------------------------------------------------------
+// Two blocks without the prefetch (the engine's form): four waves a SIMD, as attn_spec_kernel
+// (4096 prompts of 40-70 tokens, 9 / 3 heads: 220 us, with 129 registers and three waves 226).
 template <int NCB, int PF = 0>
-__global__ void __launch_bounds__(64) attn_prefill_st_kernel(
+__global__ void __launch_bounds__(64, NCB == 2 && PF == 0 ? 4 : 1) attn_prefill_st_kernel(
     const uint16_t* __restrict__ q, const int* __restrict__ cu_q, const int* __restrict__ q_start,
     const int* __restrict__ slot, const uint16_t* __restrict__ k_cache, const uint16_t* __restrict__ vt_cache,
     const uint16_t* __restrict__ pk, const uint16_t* __restrict__ pvt, int P0, int P0pad, uint16_t* __restrict__ out,
@@ -1682,19 +1686,20 @@ __global__ void __launch_bounds__(64) attn_prefill_st_kernel(
   float m[NCB], lsum[NCB];
   int own[NCB];
   bool col_valid[NCB];
-  size_t qrow[NCB];
+  uint32_t qrow[NCB];  // rows of q and out (of 128 bytes: fewer than 2^32 fit the card)
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
     const int c = 16 * cb + r16, i = c / G, g = c % G;
     col_valid[cb] = i < nq;
     own[cb] = qs + q0 + i + 1;  // causal length over own keys
-    qrow[cb] = (size_t)(qbeg + q0 + (col_valid[cb] ? i : 0)) * nh + kh * G + g;
+    qrow[cb] = (uint32_t)(qbeg + q0 + (col_valid[cb] ? i : 0)) * nh + kh * G + g;
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
-      uint4 v = *reinterpret_cast<const uint4*>(q + qrow[cb] * D + 8 * g4 + 32 * s2);
+      uint4 v = *reinterpret_cast<const uint4*>(q + (size_t)qrow[cb] * D + 8 * g4 + 32 * s2);
       if (!col_valid[cb]) v = make_uint4(0, 0, 0, 0);
       qb[cb][s2] = __builtin_bit_cast(bf16x8, v);
     }
+    asm("" : "+v"(qrow[cb]));  // kept as 32 bits: not the two registers of the row's address
 #pragma unroll
     for (int n = 0; n < 4; ++n) o[cb][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     m[cb] = -INFINITY;
@@ -1760,7 +1765,7 @@ __global__ void __launch_bounds__(64) attn_prefill_st_kernel(
   for (int cb = 0; cb < NCB; ++cb) {
     if (!col_valid[cb]) continue;
     const float inv = 1.f / lsum[cb];
-    uint16_t* orow = out + qrow[cb] * D;
+    uint16_t* orow = out + (size_t)qrow[cb] * D;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       uint2 w;
