@@ -10,8 +10,8 @@
 // once behind it (an SMS batch labels about a third of its positions).
 //
 //   forward   loss_logits<0>: a tile's logits stay in the accumulators; each row's maximum
-//             and sum of exponentials over the tile go out (8 bytes a row and tile), the label's
-//             logit from the tile that has it;
+//             and sum of exponentials over the tile's ids but the label go out (8 bytes a row and
+//             tile), the label's logit from the tile that has it;
 //             loss_join: L, loss and its mean or sum
 //   backward  per piece of the vocabulary: loss_logits<1> recomputes the tile's logits and
 //             writes d in the inputs' type; loss_grad: the piece's rows of dE, and dh's
@@ -24,6 +24,11 @@
 // type as an operand (as the gradient of such logits is under autocast); fp16 holds
 // nothing under 2^-24, so there d is scaled by 2^10 (|d| <= 1) and f takes it out.  Every
 // other sum, L and dh's shares are fp32; no float atomics, every sum has a fixed order.
+//
+// A trained model is nearly sure of most labels, and at logits of hundreds 1 - p is far below
+// L's last bit.  So L is kept in two parts, the largest logit and the logarithm of the sum over
+// it; and with t = the others' sum over the label's exponential, loss = log(1 + t) and the
+// label's d = -t / (1 + t): as exact as t, where exp(z - L) - 1 would be rounding alone.
 //
 // Products: v_mfma_f32_32x32x16, result in lane l: column l & 31 (the "lane" side: a hidden
 // row, or a vocabulary row for dE), rows (r & 3) + 8 (r >> 2) + 4 (l >> 5) (the "register"
@@ -63,8 +68,10 @@ struct LossArgs {
   const void* labels;
   uint16_t *hc, *ec, *d, *dh, *dtable;  // hc, ec, d: panels
   int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; rows, blocks done, splits
-  float *lse, *rl, *loss, *w;       // [Mp] L; [Mp] label's logit; out; [Mp] row weights or null
-  float2* part;                     // [v tiles][Mp] (maximum, sum of exp(z - maximum))
+  float *top, *ls2;                 // [Mp] x 2: L = top + ls2 ln 2
+  float *rl;                        // [Mp] label's logit, from the join on its 1 - p
+  float *loss, *w;                  // out; [Mp] row weights or null
+  float2* part;                     // [v tiles][Mp] (maximum, sum of exp(z - maximum)) without the label
   float* share;                     // [splits][Mp][Hp]
   const float *g, *gmax;            // incoming gradient; none: its largest magnitude
   long ignore;
@@ -441,15 +448,19 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
     const int vend = a.V - a.v0;
 #pragma unroll
     for (int j = 0; j < FL; ++j) {
-      // the label's logit, where this lane holds it: the same bits that the maximum and the
-      // sum are made of, so that a sure row's loss is 0 and not a rounding
+      // the label's logit, where this lane holds it, goes out and takes no part in the sum
       const int n = ln + 32 * j, y = (n < cnt ? a.lab[n] : -1) - a.v0 - rn;
       if (__any(y >= 0 && y < TR)) {
+        float zy = 0.f;
 #pragma unroll
         for (int i = 0; i < FR; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (y == 32 * i + 8 * (r >> 2) + (r & 3)) a.rl[n] = acc[i][j][r];
+          for (int r = 0; r < 16; ++r) {
+            const bool it = y == 32 * i + 8 * (r >> 2) + (r & 3);
+            zy = it ? acc[i][j][r] : zy;
+            acc[i][j][r] = it ? -INFINITY : acc[i][j][r];
+          }
+        if (y >= 0 && y < TR && !(y & 4)) a.rl[n] = zy;
       }
       float top = -INFINITY;
 #pragma unroll
@@ -487,7 +498,7 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
 #pragma unroll
     for (int j = 0; j < FL; ++j) {
       const int n = ln + 32 * j;
-      const float lse = n < cnt ? a.lse[n] : INFINITY;
+      const float top = n < cnt ? a.top[n] : INFINITY, ls2 = n < cnt ? a.ls2[n] : 0.f;
       const float w = (a.w != nullptr && n < cnt ? a.w[n] : 1.f) * (BF ? 1.f : LK_FP16);
       const int y = (n < cnt ? a.lab[n] : -1) - a.v0 - rn;  // its place in this lane's registers
       const bool here = y >= 0 && y < TR;
@@ -495,11 +506,13 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
 #pragma unroll
       for (int i = 0; i < FR; ++i) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = lk_exp(acc[i][j][r] - lse);
+        for (int r = 0; r < 16; ++r)
+          acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r] - top, LK_LOG2E, -ls2));
         if (__any(here)) {
+          const float miss = here ? a.rl[n] : 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (y == 32 * i + 8 * (r >> 2) + (r & 3)) acc[i][j][r] -= 1.f;
+            if (y == 32 * i + 8 * (r >> 2) + (r & 3)) acc[i][j][r] = -miss;
         }
         if (r0 + BR > vend) {
 #pragma unroll
@@ -598,7 +611,7 @@ __global__ void __launch_bounds__(256) loss_sum_kernel(LossArgs a) {
   lk_total(a, lk_join_blocks(a.cnt[0]), red);
 }
 
-// 16 rows a block: L from the tiles' (maximum, sum), the label's logit, the loss.  TOTAL: the
+// 16 rows a block: L from the tiles' (maximum, sum) and the label's logit, the loss.  TOTAL: the
 // block that ends last, whichever it is, takes the total too.  That saves a small call a
 // launch (5.0 us for 4.2 + 3.5), but every block's sum has to reach the others' caches: 300
 // blocks take 14.1 us with it for 4.4 + 4.3.
@@ -644,10 +657,17 @@ __global__ void __launch_bounds__(256) loss_join_kernel(LossArgs a, int tiles) {
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < 16; ++w) s += red[w][threadIdx.x].y * lk_exp_fine(red[w][threadIdx.x].x - ref);
-    float ls = logf(s);  // (not the hardware's log2: near 1 it is off by more than an ulp)
-    if (a.lab[m] == -2) ls = __builtin_nanf("");
-    loss = (top - a.rl[m]) + ls;
-    a.lse[m] = top + ls;
+    // the label joins: over the larger of both logits, e is its exponential, s the others' sum
+    // (the library's logarithms: the hardware's is off by more than an ulp near 1)
+    const float zy = a.lab[m] == -2 ? __builtin_nanf("") : a.rl[m];
+    const bool first = !(top > zy);
+    const float over = first ? zy : top, e = lk_exp_fine(zy - over);
+    if (first) s *= lk_exp_fine(top - over);
+    const float ls = first ? log1pf(s) : logf(s + e);
+    loss = (over - zy) + ls;
+    a.top[m] = over;
+    a.ls2[m] = ls * LK_LOG2E;
+    a.rl[m] = s / (s + e);
     if (a.mode == 2) a.loss[a.rows[m]] = loss;
   }
   if (a.mode == 2) return;
@@ -810,14 +830,15 @@ bool lk_bad(int N, int V, int H, int mode) {
          mode > 2 || ((long)N + 255) / 128 * (((long)V + 255) / 256) >= 1 << 24 || ((long)N + V + 512) * (H + 63) >= 1L << 34;
 }
 
-// state: ints pos[N], rows[Mp], lab[Mp], cnt[64]; floats lse[Mp], rl[Mp]
+// state: ints cnt[64], rows[Mp], lab[Mp]; floats top[Mp], ls2[Mp], rl[Mp]; ints pos[N]
 void lk_state(LossArgs& a, const LossPlan& p, void* state) {
   int* s = (int*)state;
   a.cnt = s;
   a.rows = s + 64;
   a.lab = a.rows + p.Mp;
-  a.lse = (float*)(a.lab + p.Mp);
-  a.rl = a.lse + p.Mp;
+  a.top = (float*)(a.lab + p.Mp);
+  a.ls2 = a.top + p.Mp;
+  a.rl = a.ls2 + p.Mp;
   a.pos = (int*)(a.rl + p.Mp);
   a.Mp = p.Mp, a.Hp = p.Hp, a.Vp = p.vtiles * (p.small ? 64 : 256);
   a.splits = p.splits, a.want = p.want, a.most = p.most;
@@ -837,7 +858,7 @@ int sg_loss_plan(int N, int V, int H, void* out) {
   o[0] = p.Mp;
   o[1] = p.Hp;
   o[2] = p.vtiles * (p.small ? 64 : 256);
-  o[3] = (64 + 4 * p.Mp + N + 63) / 64;
+  o[3] = (64 + 5 * p.Mp + N + 63) / 64;
   o[4] = (int)((2L * p.vtiles * p.Mp + 63) / 64);
   o[5] = (int)((64 + p.Mp + (long)p.Mp * p.piece / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
   return 0;
