@@ -35,8 +35,8 @@
 // alone its error was a third of dq's and dk's (2.8e-3 instead of 2.3e-3 of their norm at
 // 61 rows, bf16).  P and dS are rounded to the inputs' type as operands (at most 2^-8 relative
 // in bf16, as the inputs themselves are; see at_mma_p).  fp16 holds no value under 2^-24: there
-// P is scaled by 2^8 (by 2^7 forward) and dS by a power of two that the longest rows of do and
-// v set.
+// P is scaled by 2^8 (by 2^7 forward) and dS by a power of two that the longest rows of the
+// sequence's do and v set: a sequence's gradients are the same in whatever batch it is.
 //
 // What bounds it: the waves' own chains (product, exp2, rounding, product): at 16384 rows the
 // matrix units work a third of the time, the vector units half, and neither copies (10 % less
@@ -65,7 +65,7 @@ typedef __attribute__((address_space(3))) s16x4* at_tr_t;
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr float AT_LN2 = 0.6931471805599453f;
 constexpr int AT_FP16_P = 8;    // fp16: log2 of the factor on P in attn_dkv
-constexpr int AT_MAXPARTS = 256;  // fp16: blocks of each maximum
+constexpr int AT_MAXPARTS = 256;  // fp16: blocks of each maximum over the batch, but one a sequence at least
 
 __device__ const uint4 at_zero = {0, 0, 0, 0};  // what rows outside a sequence are read as
 
@@ -73,10 +73,10 @@ struct AtArgs {
   const uint16_t *q, *k, *v, *o, *dout;
   uint16_t *out, *olo, *dq, *dk, *dv;  // olo: what rounding took from o, or null (no backward)
   float *lse, *dsum, *part;   // [B, nh, Tp]: -L in log2, -D; [B, nh, T, D] x 2: dk, dv by query head
-  const float* omax;          // fp16: AT_MAXPARTS maxima of |do|^2, as many of |v|^2
+  float* omax;                // fp16: [B][2][parts] maxima of |do|^2 and of |v|^2
   const int* lens;            // [B] or null
   long qb, qh, qt, kb, kh, kt, vb, vh, vt;  // strides in elements
-  int B, T, Tp, nh, nkv, causal, split;
+  int B, T, Tp, nh, nkv, causal, split, parts;
   float scale;
 };
 
@@ -345,14 +345,14 @@ __global__ void __launch_bounds__(NW * 64) attn_fwd_kernel(AtArgs a) {
 }
 
 // fp16: the factor on dS.  dS = P (dP - D) where D is the mean of dP, so |dS| is at most half
-// of the largest |dP|, and that at most |do| |v| over the longest rows of both: the factor
-// takes this bound to 2^15, under fp16's 65504.
-__device__ __forceinline__ float at_ds_factor(const float* omax, int lane) {
+// of the largest |dP|, and that at most |do| |v| over the longest finite rows of both in the
+// sequence: the factor takes this bound to 2^15, under fp16's 65504.
+__device__ __forceinline__ float at_ds_factor(const AtArgs& a, int b, int lane) {
+  const float* m = a.omax + (size_t)b * 2 * a.parts;
   float x = 0.f, y = 0.f;
-#pragma unroll
-  for (int i = 0; i < AT_MAXPARTS / 64; ++i) {
-    x = fmaxf(x, omax[lane + 64 * i]);
-    y = fmaxf(y, omax[AT_MAXPARTS + lane + 64 * i]);
+  for (int i = lane; i < a.parts; i += 64) {
+    x = fmaxf(x, m[i]);
+    y = fmaxf(y, m[a.parts + i]);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -365,29 +365,25 @@ __device__ __forceinline__ float at_ds_factor(const float* omax, int lane) {
   return __uint_as_float((uint32_t)(127 + 15 - (e >> 1)) << 23);
 }
 
-// The largest squared length of do's (y = 0) and v's (y = 1) rows of a head inside the
-// sequences: what lies behind them must not move the factor.  D / 8 lanes a row.
+// The largest squared length of do's (y = 0) and v's (y = 1) finite rows of a head, sequence by
+// sequence: neither what lies behind a sequence, nor another one, nor an infinity (a matter of
+// the rows that meet it) moves the factor.  D / 8 lanes a row; block part of `parts`.
 template <int D>
 __global__ void __launch_bounds__(1024) attn_omax_kernel(AtArgs a) {
   __shared__ float red[16];
   const bool isv = blockIdx.y == 1;
-  const int heads = isv ? a.nkv : a.nh;
-  const long rows = (long)heads * a.T, n = a.B * rows * (D / 8);
-  // (64-bit divisions cost most of the kernel; almost every batch does without)
-  auto div = [&](long x, long y) { return n >> 32 ? x / y : (long)((uint32_t)x / (uint32_t)y); };
+  const int b = blockIdx.x / a.parts, part = blockIdx.x - b * a.parts;
+  const int len = a.lens != nullptr ? min(max(a.lens[b], 0), a.T) : a.T;
+  const uint16_t* src = isv ? a.v + b * a.vb : a.dout + (size_t)b * a.T * a.nh * D;
+  const long n = (long)len * (isv ? a.nkv : a.nh) * (D / 8);
   float m = 0.f;
-  for (long i = (long)blockIdx.x * 1024 + threadIdx.x; i < n; i += (long)AT_MAXPARTS * 1024) {
-    const long r = i / (D / 8), b = div(r, rows), j = r - b * rows;
+  for (long i = (long)part * 1024 + threadIdx.x; i < n; i += (long)a.parts * 1024) {
+    const long r = i / (D / 8);
     const int c = (int)(i % (D / 8)) * 8;
-    const int len = a.lens != nullptr ? min(max(a.lens[b], 0), a.T) : a.T;
-    const uint16_t* p;
-    if (isv) {
-      const long g = div(j, a.T), t = j - g * a.T;
-      if (t >= len) continue;
-      p = a.v + b * a.vb + g * a.vh + t * a.vt + c;
-    } else {
-      if (j >= (long)len * heads) continue;
-      p = a.dout + r * D + c;
+    const uint16_t* p = src + r * D + c;
+    if (isv) {  // (64-bit divisions cost most of the kernel; almost every batch does without)
+      const long g = n >> 32 ? r / len : (long)((uint32_t)r / (uint32_t)len);
+      p = src + g * a.vh + (r - g * len) * a.vt + c;
     }
     const f16x8 v = *reinterpret_cast<const f16x8*>(p);
     float s = 0.f;
@@ -395,7 +391,7 @@ __global__ void __launch_bounds__(1024) attn_omax_kernel(AtArgs a) {
     for (int k = 0; k < 8; ++k) s = fmaf((float)v[k], (float)v[k], s);
 #pragma unroll
     for (int o = 1; o < D / 8; o <<= 1) s += __shfl_xor(s, o, 64);
-    m = fmaxf(m, s);
+    if (s < INFINITY) m = fmaxf(m, s);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
@@ -403,7 +399,7 @@ __global__ void __launch_bounds__(1024) attn_omax_kernel(AtArgs a) {
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w]);
-    const_cast<float*>(a.omax)[blockIdx.y * AT_MAXPARTS + blockIdx.x] = m;
+    a.omax[((size_t)b * 2 + blockIdx.y) * a.parts + part] = m;
   }
 }
 
@@ -450,7 +446,7 @@ __global__ void __launch_bounds__(NW * 64) attn_dq_kernel(AtArgs a) {
   const float lse = on ? a.lse[(size_t)bh * a.Tp + qr] : -INFINITY;  // -L
   const float c = a.scale * AT_LOG2E;
   float dsf = 1.f;
-  if constexpr (!BF) dsf = at_ds_factor(a.omax, lane);
+  if constexpr (!BF) dsf = at_ds_factor(a, b, lane);
   f32x16 dq[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) dq[dt] = (f32x16)0.f;
@@ -537,7 +533,7 @@ __global__ void __launch_bounds__(NW * 64) attn_dkv_kernel(AtArgs a) {
   at_own<D>(vf, a.v + b * a.vb + g * a.vh + kr * a.vt, on, h);
   const float c = a.scale * AT_LOG2E;
   float dsf = 1.f;
-  if constexpr (!BF) dsf = at_ds_factor(a.omax, lane) * (1.f / (1 << AT_FP16_P));
+  if constexpr (!BF) dsf = at_ds_factor(a, b, lane) * (1.f / (1 << AT_FP16_P));
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = (f32x16)0.f;
@@ -649,6 +645,12 @@ bool at_bad(int B, int T, int nh, int nkv, int D) {
          (long)B * nh > (1 << 20) || ((long)T + 127) / 128 * B * nh >= 1 << 24;  // (a grid holds 2^32 threads)
 }
 
+int at_parts(int B) {
+  int p = AT_MAXPARTS;
+  while (p > 1 && p * B > AT_MAXPARTS) p >>= 1;
+  return p;
+}
+
 template <bool BF, int D>
 void at_launch_fwd(const AtArgs& a, hipStream_t st) {
   const int pairs = a.B * a.nh;
@@ -663,7 +665,7 @@ void at_launch_fwd(const AtArgs& a, hipStream_t st) {
 template <bool BF, int D>
 void at_launch_bwd(const AtArgs& a, hipStream_t st) {
   const int pairs = a.B * a.nh, kpairs = a.B * (a.split ? a.nh : a.nkv);
-  if constexpr (!BF) attn_omax_kernel<D><<<dim3(AT_MAXPARTS, 2), dim3(1024), 0, st>>>(a);
+  if constexpr (!BF) attn_omax_kernel<D><<<dim3(a.B * a.parts, 2), dim3(1024), 0, st>>>(a);
   if (a.T <= 32) {
     attn_dq_kernel<BF, D, 1><<<dim3((a.Tp + 31) / 32 * pairs), dim3(64), 0, st>>>(a);
     attn_dkv_kernel<BF, D, 1><<<dim3((a.T + 31) / 32 * kpairs), dim3(64), 0, st>>>(a);
@@ -693,6 +695,9 @@ int sg_attn_split(int B, int T, int nh, int nkv) {
   return nh != nkv && (long)B * nkv * ((T + 127) / 128) < 1024 && T > 128 ? 1 : 0;
 }
 
+// fp16: floats of the maxima that the factors on dS come from.
+int sg_attn_maxima(int B) { return (2 * B * at_parts(B) + 63) / 64 * 64; }
+
 int sg_attn_fwd(const void* q, const void* k, const void* v, const void* lens, void* out, void* olo, void* lse,
                 const void* strides,
                 int B, int T, int nh, int nkv, int D, int causal, int fp16, float scale, hipStream_t st) {
@@ -710,7 +715,7 @@ int sg_attn_fwd(const void* q, const void* k, const void* v, const void* lens, v
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-// ws: fp32 [B nh rows] (D), then 512 (fp16 only), then [2][B, nh, T, D] where sg_attn_split
+// ws: fp32 [B nh rows] (D), then sg_attn_maxima (fp16 only), then [2][B, nh, T, D] where sg_attn_split
 int sg_attn_bwd(const void* q, const void* k, const void* v, const void* lens, const void* out, const void* olo,
                 const void* lse, const void* dout, void* dq, void* dk, void* dv, void* ws, const void* strides, int B, int T, int nh,
                 int nkv, int D, int causal, int fp16, float scale, hipStream_t st) {
@@ -727,7 +732,8 @@ int sg_attn_bwd(const void* q, const void* k, const void* v, const void* lens, c
   float* w = a.dsum + (size_t)B * nh * a.Tp;
   if (fp16) {
     a.omax = w;
-    w += 2 * AT_MAXPARTS;
+    a.parts = at_parts(B);
+    w += sg_attn_maxima(B);
   }
   a.part = w;
   if (fp16)

@@ -154,7 +154,7 @@ struct Attention : torch::autograd::Function<Attention> {
       dk = at::empty(k.sizes(), k.options());
       dv = at::empty(v.sizes(), v.options());
       const bool split = sg_attn_split(s.B, s.T, s.nh, s.nkv);
-      const Tensor ws = words(q, s.stats + 512 * s.fp16 + (split ? 2L * s.B * s.nh * s.T * s.D : 0));
+      const Tensor ws = words(q, s.stats + (s.fp16 ? sg_attn_maxima(s.B) : 0) + (split ? 2L * s.B * s.nh * s.T * s.D : 0));
       float* lse = keep.data_ptr<float>();
       run(q, "attn_bwd", sg_attn_bwd, ptr(q), ptr(k), ptr(v), ptr(saved[3]), ptr(out), (const void*)(lse + s.stats),
           (const void*)lse, ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(ws), (const void*)s.strides, s.B, s.T, s.nh, s.nkv,

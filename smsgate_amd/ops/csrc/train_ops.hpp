@@ -16,6 +16,7 @@ int sg_embed_grad(const void* ids, const void* add, int is64, const void* dx, vo
 // attn_grad_kernels.hip.  strides: of q, k and v, in elements: batch, head, row
 int sg_attn_rows(int T);
 int sg_attn_split(int B, int T, int nh, int nkv);
+int sg_attn_maxima(int B);
 int sg_attn_fwd(const void* q, const void* k, const void* v, const void* lens, void* out, void* olo, void* lse,
                 const void* strides, int B, int T, int nh, int nkv, int D, int causal, int fp16, float scale,
                 hipStream_t st);
