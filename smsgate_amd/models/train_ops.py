@@ -245,8 +245,9 @@ def embed_lookup(ids: torch.Tensor, table: torch.Tensor, add_ids: Optional[torch
         raise TypeError("embed_lookup: ids must be int32 or int64")
     if add_ids is not None and (add_ids.shape != ids.shape or add_ids.dtype != ids.dtype):
         raise ValueError("embed_lookup: add_ids must have the shape and type of ids")
-    if not (1 <= table.shape[0] < 1 << 26 and 1 <= table.shape[1] <= 1 << 20) or ids.numel() >= 1 << 26:
-        raise ValueError("embed_lookup: 1 <= V < 2^26, 1 <= H <= 2^20, fewer than 2^26 ids")
+    most = (1 << 26) - 4  # a wave a row, 4 a block, fewer than 2^32 threads
+    if not (1 <= table.shape[0] <= most and 1 <= table.shape[1] <= 1 << 20) or ids.numel() > most:
+        raise ValueError("embed_lookup: 1 <= V <= 2^26 - 4, 1 <= H <= 2^20, at most 2^26 - 4 ids")
     _on_gpu("embed_lookup", table, ids, add_ids)
     return _native().embed(table, ids, add_ids, float(scale))
 

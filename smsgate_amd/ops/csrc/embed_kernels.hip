@@ -517,9 +517,10 @@ int eg_backward(const void* ids, const void* add, int is64, const void* dx, void
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-// (a grid holds 2^32 threads: 64 a row of x, 64 a row of dE)
+// (64 threads a row of x and a row of dE, 256 a block, and a grid holds 2^32 - 1)
+constexpr int EG_MOST = (1 << 26) - 4;
 bool eg_bad(int n, int V, int H, int dtype, int vec) {
-  return n <= 0 || n >= (1 << 26) || V <= 0 || V >= (1 << 26) || H <= 0 || H > (1 << 20) || dtype < 0 || dtype > 2 ||
+  return n <= 0 || n > EG_MOST || V <= 0 || V > EG_MOST || H <= 0 || H > (1 << 20) || dtype < 0 || dtype > 2 ||
          (vec && H % (dtype == 0 ? 4 : 8));
 }
 
