@@ -214,7 +214,7 @@ def load_train_autograd():
         load_library()  # its entries, and built together
         if _build.needs_build_autograd():
             _build.build_autograd()
-        spec = importlib.util.spec_from_file_location(_build.AUTOGRAD.stem, _build.AUTOGRAD)
+        spec = importlib.util.spec_from_file_location(_build.AUTOGRAD_NAME, _build.AUTOGRAD)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
         _train_autograd = mod

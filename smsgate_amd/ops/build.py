@@ -8,9 +8,10 @@ takes the caller's ``hipStream_t`` so it can be captured into a hipGraph.
 The build is skipped when the .so is newer than all sources.
 
 One part is built against torch's headers: ``csrc/train_autograd.cpp``, the training
-operators' autograd functions, into ``_lib/smsgate_train_autograd.so``.  A small training call
-is host time, and a Python Function costs more of it than all its kernels.  It links the
-kernel library, whose entries keep their C ABI.
+operators' autograd functions, into ``_lib/smsgate_train_autograd.torch-<version>.<interpreter>.so``
+(a file for each that it is compiled against).  A small training call is host time, and a
+Python Function costs more of it than all its kernels.  It links the kernel library, whose
+entries keep their C ABI.
 """
 from __future__ import annotations
 
@@ -22,12 +23,15 @@ import sysconfig
 from pathlib import Path
 from typing import List, Optional
 
+import torch
+
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIBDIR = HERE / "_lib"
 LIB = LIBDIR / "libsmsgate_kernels.so"
 AUTOGRAD_SRC = CSRC / "train_autograd.cpp"
-AUTOGRAD = LIBDIR / "smsgate_train_autograd.so"
+AUTOGRAD_NAME = "smsgate_train_autograd"
+AUTOGRAD = LIBDIR / f"{AUTOGRAD_NAME}.torch-{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX') or '.so'}"
 ARCH = os.environ.get("SMSGATE_OFFLOAD_ARCH", "gfx950")
 # what every HIP source is compiled with
 FLAGS = [
@@ -62,18 +66,25 @@ def sources() -> List[Path]:
     return sorted(CSRC.glob("*.hip"))
 
 
+def _older(built: Path, deps: List[Path]) -> bool:
+    return not built.exists() or any(d.stat().st_mtime > built.stat().st_mtime for d in deps)
+
+
+def _tmp(built: Path) -> Path:
+    """Where ``built`` is written until it is whole: a file of this process, as the ranks of a
+    job may build at once."""
+    return built.with_name(f"{built.name}.{os.getpid()}.tmp")
+
+
 def needs_build(lib: Path = LIB) -> bool:
-    if not lib.exists():
-        return True
-    mt = lib.stat().st_mtime
-    return any(s.stat().st_mtime > mt for s in sources() + [Path(__file__)])
+    return _older(lib, sources() + sorted(CSRC.glob("*.hpp")) + [Path(__file__)])
 
 
 def build(force: bool = False, verbose: bool = False, extra: Optional[List[str]] = None) -> Path:
     if not force and not needs_build():
         return LIB
     LIBDIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB.with_suffix(".so.tmp")
+    tmp = _tmp(LIB)
     cmd = [
         hipcc(),
         *FLAGS,
@@ -91,10 +102,7 @@ def build(force: bool = False, verbose: bool = False, extra: Optional[List[str]]
 
 
 def needs_build_autograd() -> bool:
-    if not AUTOGRAD.exists():
-        return True
-    mt = AUTOGRAD.stat().st_mtime
-    return any(s.stat().st_mtime > mt for s in (AUTOGRAD_SRC, CSRC / "train_ops.hpp"))
+    return _older(AUTOGRAD, [AUTOGRAD_SRC, *sorted(CSRC.glob("*.hpp")), Path(__file__)])
 
 
 def build_autograd(force: bool = False, verbose: bool = False) -> Path:
@@ -102,10 +110,8 @@ def build_autograd(force: bool = False, verbose: bool = False) -> Path:
     library it links."""
     if not force and not needs_build_autograd():
         return AUTOGRAD
-    import torch
-
     root = Path(torch.__file__).resolve().parent
-    tmp = AUTOGRAD.with_suffix(".so.tmp")
+    tmp = _tmp(AUTOGRAD)
     cmd = [
         os.environ.get("CXX", "g++"),
         "-O2",
@@ -114,7 +120,7 @@ def build_autograd(force: bool = False, verbose: bool = False) -> Path:
         "-shared",
         "-D__HIP_PLATFORM_AMD__=1",  # torch's and HIP's headers on ROCm ask for both
         "-DUSE_ROCM=1",
-        f"-DTORCH_EXTENSION_NAME={AUTOGRAD.stem}",
+        f"-DTORCH_EXTENSION_NAME={AUTOGRAD_NAME}",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         *(x for d in (root / "include", root / "include/torch/csrc/api/include",
                       Path(hipcc()).resolve().parent.parent / "include", sysconfig.get_paths()["include"])
