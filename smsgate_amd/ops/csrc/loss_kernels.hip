@@ -21,7 +21,8 @@
 // Four products of 2 n V H flops where keeping the logits would need three: z is needed in
 // fp32 (its rounding to 16 bits would put errors of per cents into exp), and storing it
 // costs more memory time at H = 576 than multiplying again.  d is rounded to the inputs'
-// type as an operand (as the gradient of such logits is under autocast); fp16 holds
+// type as an operand (as the gradient of such logits is under autocast; up to 128 rows what
+// rounding took is a second operand); fp16 holds
 // nothing under 2^-24, so there d is scaled by 2^10 (|d| <= 1) and f takes it out.  Every
 // other sum, L and dh's shares are fp32; no float atomics, every sum has a fixed order.
 //
@@ -67,6 +68,7 @@ struct LossArgs {
   const uint16_t *h, *table;
   const void* labels;
   uint16_t *hc, *ec, *d, *dh, *dtable;  // hc, ec, d: panels
+  long lo;                          // few rows: what rounding took from d lies so far behind it, else 0
   int *pos, *rows, *lab, *cnt;      // [N] place or -1; [Mp] row of a place; [Mp] label; rows, blocks done, splits
   float *top, *ls2;                 // [Mp] x 2: L = top + ls2 ln 2
   float *rl;                        // [Mp] label's logit, from the join on its 1 - p
@@ -101,6 +103,15 @@ __device__ __forceinline__ uint16_t lk_round(float x) {
     const _Float16 b = (_Float16)x;
     return __builtin_bit_cast(uint16_t, b);
   }
+}
+
+// x without what rounding to the type keeps of it
+template <bool BF>
+__device__ __forceinline__ float lk_rest(float x) {
+  if constexpr (BF)
+    return x - (float)(__bf16)x;
+  else
+    return x - (float)(_Float16)x;
 }
 
 template <bool BF>
@@ -338,17 +349,19 @@ __device__ int lk_choose(const LossArgs& a, int cnt, int lane) {
 // MODE 2: lane = the piece's vocabulary rows, register = H, k = hidden rows.
 // MODE 3: lane = hidden rows, register = H, k = a split of the piece.
 // 32 k-values a step, ST buffers: the copies of the next ST - 1 steps are in flight.
-template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST>
+// FINE: d is two operands, its rounding and what that took, a tile of each in every step.
+template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST, bool FINE>
 struct LkTile {
   static constexpr int NW = WL * WR, TL = BL / WL, TR = BR / WR, FL = TL / 32, FR = TR / 32;
-  static constexpr int BK = LK_PANEL, STAGE = (BL + BR) * BK, NI = (BL + BR) / 16 / NW;
+  static constexpr int LT = FINE && MODE >= 2 ? 2 : 1;  // lane-side tiles a step
+  static constexpr int BK = LK_PANEL, STAGE = (LT * BL + BR) * BK, NI = (LT * BL + BR) / 16 / NW;
   static_assert(ST * STAGE * 2 <= 160 * 1024 && BL % (32 * WL) == 0 && BR % (32 * WR) == 0, "tile");
   static __device__ __forceinline__ void run(const LossArgs& a, int block, uint16_t* sm);
 };
 
-template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST>
-__device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const LossArgs& a, int block,
-                                                                          uint16_t* sm) {
+template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST, bool FINE>
+__device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST, FINE>::run(const LossArgs& a, int block,
+                                                                                uint16_t* sm) {
   constexpr bool LCOL = MODE == 2, RCOL = MODE >= 2;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int wl = wave / WR, wr = wave % WR;
@@ -382,17 +395,21 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
   const uint32_t lane_off = (lane >> 2) * 64 + (((lane & 3) ^ lk_swz(lane >> 2)) << 4);
   const long mpan = (long)a.Mp * LK_PANEL, vpan = (long)a.Vp * LK_PANEL;  // a panel of hc or d, of ec
   auto stage = [&](int k0, int buf) {
-    uint16_t *ls = sm + buf * STAGE, *rs = ls + BL * BK;
+    uint16_t *ls = sm + buf * STAGE, *rs = ls + LT * BL * BK;
     const int kp = k0 / LK_PANEL;
     if constexpr (MODE <= 1) {
       lk_stage<BL, NW, false>(a.hc + kp * mpan + (long)l0 * LK_PANEL, 0, 0, ls, wave, lane_off);
       lk_stage<BR, NW, false>(a.ec + kp * vpan + (long)(a.v0 + r0) * LK_PANEL, 0, 0, rs, wave, lane_off);
     } else if constexpr (MODE == 2) {
-      lk_stage<BL, NW, true>(a.d + l0 / LK_PANEL * mpan + (long)k0 * LK_PANEL, mpan, BL / 32, ls, wave, lane_off);
+      const uint16_t* d = a.d + l0 / LK_PANEL * mpan + (long)k0 * LK_PANEL;
+#pragma unroll
+      for (int t = 0; t < LT; ++t) lk_stage<BL, NW, true>(d + t * a.lo, mpan, BL / 32, ls + t * BL * BK, wave, lane_off);
       lk_stage<BR, NW, true>(a.hc + r0 / LK_PANEL * mpan + (long)k0 * LK_PANEL, mpan, (a.Hp - r0) / LK_PANEL, rs, wave,
                              lane_off);
     } else {
-      lk_stage<BL, NW, false>(a.d + kp * mpan + (long)l0 * LK_PANEL, 0, 0, ls, wave, lane_off);
+      const uint16_t* d = a.d + kp * mpan + (long)l0 * LK_PANEL;
+#pragma unroll
+      for (int t = 0; t < LT; ++t) lk_stage<BL, NW, false>(d + t * a.lo, 0, 0, ls + t * BL * BK, wave, lane_off);
       lk_stage<BR, NW, true>(a.ec + r0 / LK_PANEL * vpan + (long)(a.v0 + k0) * LK_PANEL, vpan, (a.Hp - r0) / LK_PANEL,
                              rs, wave, lane_off);
     }
@@ -416,15 +433,17 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (k0 + (ST - 1) * BK < ke) stage(k0 + (ST - 1) * BK, buf == 0 ? ST - 1 : buf - 1);
-    const uint16_t *ls = sm + buf * STAGE, *rs = ls + BL * BK;
+    const uint16_t *ls = sm + buf * STAGE, *rs = ls + LT * BL * BK;
     buf = buf + 1 == ST ? 0 : buf + 1;
     // the operands of the next 16 k-values are read while these are multiplied
-    u16x8 lf[2][FL], rf[2][FR];
+    u16x8 lf[2][LT][FL], rf[2][FR];
     auto read = [&](int s) {
 #pragma unroll
-      for (int j = 0; j < FL; ++j)
-        lf[s & 1][j] = LCOL ? lk_col(ls + (wl * FL + j) * 32 * LK_PANEL, s, lane)
-                            : lk_row(ls, wl * TL + 32 * j + (lane & 31), s, h);
+      for (int t = 0; t < LT; ++t)
+#pragma unroll
+        for (int j = 0; j < FL; ++j)
+          lf[s & 1][t][j] = LCOL ? lk_col(ls + t * BL * BK + (wl * FL + j) * 32 * LK_PANEL, s, lane)
+                                 : lk_row(ls + t * BL * BK, wl * TL + 32 * j + (lane & 31), s, h);
 #pragma unroll
       for (int i = 0; i < FR; ++i)
         rf[s & 1][i] = RCOL ? lk_col(rs + (wr * FR + i) * 32 * LK_PANEL, s, lane)
@@ -437,7 +456,9 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
 #pragma unroll
       for (int i = 0; i < FR; ++i)
 #pragma unroll
-        for (int j = 0; j < FL; ++j) acc[i][j] = lk_mma<BF>(rf[s & 1][i], lf[s & 1][j], acc[i][j]);
+        for (int j = 0; j < FL; ++j)
+#pragma unroll
+          for (int t = 0; t < LT; ++t) acc[i][j] = lk_mma<BF>(rf[s & 1][i], lf[s & 1][t][j], acc[i][j]);
     }
   }
   // register r of acc[i][j]: register-side index r0 + wr TR + 32 i + 8 (r >> 2) + 4 h + (r & 3)
@@ -520,9 +541,16 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
             if (rn + 32 * i + 8 * (r >> 2) + (r & 3) >= vend) acc[i][j][r] = 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 4; e += 2)
-          *reinterpret_cast<uint4*>(row + i * mpan + 8 * (e + h)) =
-              lk_trade<BF>(lk_four(acc[i][j], e, w), lk_four(acc[i][j], e + 1, w));
+        for (int e = 0; e < 4; e += 2) {
+          float4 x = lk_four(acc[i][j], e, w), y = lk_four(acc[i][j], e + 1, w);
+          uint16_t* at = row + i * mpan + 8 * (e + h);
+          *reinterpret_cast<uint4*>(at) = lk_trade<BF>(x, y);
+          if constexpr (FINE) {
+            x = make_float4(lk_rest<BF>(x.x), lk_rest<BF>(x.y), lk_rest<BF>(x.z), lk_rest<BF>(x.w));
+            y = make_float4(lk_rest<BF>(y.x), lk_rest<BF>(y.y), lk_rest<BF>(y.z), lk_rest<BF>(y.w));
+            *reinterpret_cast<uint4*>(at + a.lo) = lk_trade<BF>(x, y);
+          }
+        }
       }
     }
   } else {
@@ -557,9 +585,9 @@ __device__ __forceinline__ void LkTile<BF, MODE, BL, BR, WL, WR, ST>::run(const 
   }
 }
 
-template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST>
-__global__ void __launch_bounds__(WL * WR * 64, 3) loss_logits_kernel(LossArgs a) {
-  typedef LkTile<BF, MODE, BL, BR, WL, WR, ST> Tile;
+template <bool BF, int MODE, int BL, int BR, int WL, int WR, int ST, bool FINE>
+__global__ void __launch_bounds__(WL * WR * 64, FINE ? 2 : 3) loss_logits_kernel(LossArgs a) {
+  typedef LkTile<BF, MODE, BL, BR, WL, WR, ST, FINE> Tile;
   __shared__ __attribute__((aligned(16))) uint16_t sm[ST * Tile::STAGE];
   Tile::run(a, blockIdx.x, sm);
 }
@@ -567,10 +595,10 @@ __global__ void __launch_bounds__(WL * WR * 64, 3) loss_logits_kernel(LossArgs a
 // dE's tiles (the first a.t2 blocks), then dh's: one launch, because neither fills the card
 // by itself (16384 ids and 576 columns: 384 tiles for 512 places) and dh's, split as finely
 // as one likes, fill the places that dE's leave.
-template <bool BF, int BL, int BR, int WL, int WR, int ST>
+template <bool BF, int BL, int BR, int WL, int WR, int ST, bool FINE>
 __global__ void __launch_bounds__(WL * WR * 64, 3) loss_grad_kernel(LossArgs a) {
-  typedef LkTile<BF, 2, BL, BR, WL, WR, ST> Table;
-  typedef LkTile<BF, 3, BL, BR, WL, WR, ST> Hidden;
+  typedef LkTile<BF, 2, BL, BR, WL, WR, ST, FINE> Table;
+  typedef LkTile<BF, 3, BL, BR, WL, WR, ST, FINE> Hidden;
   __shared__ __attribute__((aligned(16))) uint16_t sm[ST * Table::STAGE];
   if ((int)blockIdx.x < a.t2)
     Table::run(a, blockIdx.x, sm);
@@ -737,8 +765,15 @@ __global__ void __launch_bounds__(256) loss_dh_kernel(LossArgs a) {
 // Big tiles (256 x 256, 8 waves) read 3 KB of LDS per 4 products; a few hundred rows leave
 // most of the card without one, so there 64 x 64 tiles of 4 waves run instead.
 struct LossPlan {
-  int Mp, Hp, small, vtiles, piece, splits, want, most;
+  int Mp, Hp, small, fine, vtiles, piece, splits, want, most;
 };
+
+// Rows up to which d is two operands.  Its rounding adds to the gradients' own (sqrt 2 of it
+// over many rows); of few rows, each with its label's term, one rounding shows as it is: 1.5 to
+// 2.2 of the gradient's own for a third of the calls of one row, a tenth of those of 5 and a
+// thirtieth of those of 64, none of 120 from 128 rows on.  The gradients of 61 rows, 8192 x 256,
+// take 8.1 us for 7.6, a whole call of 128 rows, 49152 x 576, 139 us for 125.
+constexpr int LK_FINE = 128;
 
 constexpr int LK_BL = 128;  // lane side of the gradients' big tiles
 constexpr long LK_PIECE = 1L << 27;  // elements of d (256 MB: what the last-level cache holds)
@@ -748,9 +783,10 @@ LossPlan lk_plan(int N, int V, int H) {
   p.Mp = (N + LK_PAD - 1) / LK_PAD * LK_PAD;
   p.Hp = (H + LK_K - 1) / LK_K * LK_K;
   const long vp = ((long)V + LK_PAD - 1) / LK_PAD * LK_PAD;
+  p.fine = N <= LK_FINE;
   p.small = (p.Mp / 256) * (vp / 256) < 256;
   p.vtiles = (int)(vp / (p.small ? 64 : 256));
-  long piece = LK_PIECE / p.Mp / LK_PAD * LK_PAD;
+  long piece = LK_PIECE / (1 + p.fine) / p.Mp / LK_PAD * LK_PAD;
   if (piece < 4 * LK_PAD) piece = 4 * LK_PAD;
   p.piece = (int)(piece < vp ? piece : vp);
   // dh: blocks over the card, each with at least 4 steps of k
@@ -765,10 +801,16 @@ LossPlan lk_plan(int N, int V, int H) {
 
 template <bool BF, int MODE>
 void lk_logits(const LossArgs& a, const LossPlan& p, hipStream_t st) {
-  if (p.small)
-    loss_logits_kernel<BF, MODE, 64, 64, 2, 2, 4><<<dim3(a.Mp / 64 * (a.vn / 64)), dim3(256), 0, st>>>(a);
+  const dim3 grid = p.small ? a.Mp / 64 * (a.vn / 64) : a.Mp / 128 * (a.vn / 256);
+  constexpr bool FINE = MODE == 1;
+  if (p.small && p.fine && FINE)
+    loss_logits_kernel<BF, MODE, 64, 64, 2, 2, 4, FINE><<<grid, dim3(256), 0, st>>>(a);
+  else if (p.small)
+    loss_logits_kernel<BF, MODE, 64, 64, 2, 2, 4, false><<<grid, dim3(256), 0, st>>>(a);
+  else if (p.fine && FINE)
+    loss_logits_kernel<BF, MODE, 128, 256, 1, 4, 2, FINE><<<grid, dim3(256), 0, st>>>(a);
   else
-    loss_logits_kernel<BF, MODE, 128, 256, 1, 4, 2><<<dim3(a.Mp / 128 * (a.vn / 256)), dim3(256), 0, st>>>(a);
+    loss_logits_kernel<BF, MODE, 128, 256, 1, 4, 2, false><<<grid, dim3(256), 0, st>>>(a);
 }
 
 // dh has as many blocks as any count of rows may want (its tiles' rows x splits are at most the
@@ -782,10 +824,14 @@ void lk_grads(LossArgs a, const LossPlan& p, hipStream_t st) {
   }
   if (a.t2 + t3 == 0) return;
   const dim3 grid((unsigned)(a.t2 + t3));
-  if (p.small)
-    loss_grad_kernel<BF, 64, 64, 2, 2, 4><<<grid, dim3(256), 0, st>>>(a);
+  if (p.small && p.fine)
+    loss_grad_kernel<BF, 64, 64, 2, 2, 4, true><<<grid, dim3(256), 0, st>>>(a);
+  else if (p.fine)
+    loss_grad_kernel<BF, LK_BL, 192, 4, 1, 2, true><<<grid, dim3(256), 0, st>>>(a);
+  else if (p.small)
+    loss_grad_kernel<BF, 64, 64, 2, 2, 4, false><<<grid, dim3(256), 0, st>>>(a);
   else
-    loss_grad_kernel<BF, LK_BL, 192, 4, 1, 2><<<grid, dim3(256), 0, st>>>(a);
+    loss_grad_kernel<BF, LK_BL, 192, 4, 1, 2, false><<<grid, dim3(256), 0, st>>>(a);
 }
 
 template <bool BF>
@@ -842,6 +888,7 @@ void lk_state(LossArgs& a, const LossPlan& p, void* state) {
   a.pos = (int*)(a.rl + p.Mp);
   a.Mp = p.Mp, a.Hp = p.Hp, a.Vp = p.vtiles * (p.small ? 64 : 256);
   a.splits = p.splits, a.want = p.want, a.most = p.most;
+  a.lo = p.fine ? (long)p.Mp * p.piece : 0;
   a.bl = p.small ? 64 : LK_BL, a.nr = p.small ? (a.H + 63) / 64 : (a.H + 191) / 192;
 }
 
@@ -860,7 +907,7 @@ int sg_loss_plan(int N, int V, int H, void* out) {
   o[2] = p.vtiles * (p.small ? 64 : 256);
   o[3] = (64 + 5 * p.Mp + N + 63) / 64;
   o[4] = (int)((2L * p.vtiles * p.Mp + 63) / 64);
-  o[5] = (int)((64 + p.Mp + (long)p.Mp * p.piece / 2 + (long)p.splits * p.Mp * p.Hp + 63) / 64);
+  o[5] = (int)((64 + p.Mp + (long)p.Mp * p.piece / 2 * (1 + p.fine) + (long)p.splits * p.Mp * p.Hp + 63) / 64);
   return 0;
 }
 
@@ -892,7 +939,7 @@ int sg_loss_bwd(const void* hc, const void* ec, void* state, const void* g, void
   a.gmax = w;
   a.w = mode == 2 ? w + 64 : nullptr;
   a.d = (uint16_t*)(w + 64 + p.Mp);
-  a.share = w + 64 + p.Mp + (size_t)p.Mp * p.piece / 2;
+  a.share = w + 64 + p.Mp + (size_t)p.Mp * p.piece / 2 * (1 + p.fine);
   fp16 ? lk_backward<false>(a, p, st) : lk_backward<true>(a, p, st);
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
