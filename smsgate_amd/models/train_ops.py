@@ -31,8 +31,12 @@ Three operators of the whole step, on request (``hip_ops``; TrainConfig.hip_ops)
   span answer formats (csrc/loss_kernels.hip).
 
 Their autograd functions are C++ (csrc/train_autograd.cpp): one message's call is host time,
-and a Python Function spends 1.3 times as much of it (45 positions forward and backward 36 ->
-26 us, attention of 37 rows 57 -> 40, the loss of 61 rows 60 -> 47).
+and a Python Function spends 1.3 to 1.7 times as much of it.  Forward and backward of 45
+positions take 26 to 46 us (36 to 79 in Python), attention of 37 rows 40 to 70 (57 to 116),
+the loss of 61 rows 47 to 76 (60 to 115): autograd hands a GPU backward to another thread and
+back in about 16 us or in 40, for seconds at a time.  Through autograd, torch's own operators
+take 46 us for the embedding, 104 for the attention and 170 for the loss where these take 45,
+64 and 73.
 
 Their forward and backward can be captured into a graph.  As with any torch operator, no
 eager graph of the same leaves may be alive then: a leaf's accumulation node belongs to the
@@ -266,7 +270,9 @@ def tiled_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
     ``scale``: > 0, default ``D ** -0.5``.  ``causal``: query i sees keys up to i.
     ``lengths`` (int32 [B]): sequence b is its first ``lengths[b]`` rows (clamped to 0..T);
     the rows behind are zero in the result and in every gradient, and what they hold in q,
-    k, v and the incoming gradient has no effect, infinities and NaN included.  Returns
+    k, v and the incoming gradient has no effect, infinities and NaN included.  (Inside a
+    sequence, an infinity or NaN may reach rows that a causal mask keeps from it, as 0 times
+    it does in any product with masked probabilities; other sequences never.)  Returns
     [B, T, nh * D] (the o-projection's input).  Probabilities are recomputed in the
     backward pass and nothing of size T x T is stored; every sum has a fixed order."""
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:

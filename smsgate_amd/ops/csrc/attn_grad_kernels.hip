@@ -36,7 +36,7 @@
 // 61 rows, bf16).  P and dS are rounded to the inputs' type as operands (at most 2^-8 relative
 // in bf16, as the inputs themselves are; see at_mma_p).  fp16 holds no value under 2^-24: there
 // P is scaled by 2^8 (by 2^7 forward) and dS by a power of two that the longest rows of the
-// sequence's do and v set: a sequence's gradients are the same in whatever batch it is.
+// sequence's do and v set (and nothing in another sequence).
 //
 // What bounds it: the waves' own chains (product, exp2, rounding, product): at 16384 rows the
 // matrix units work a third of the time, the vector units half, and neither copies (10 % less

@@ -42,8 +42,9 @@
 // less time with the copies left out, none with LDS reads or exp left out), and that a block's
 // waves wait together: three blocks a CU of 128 x 256 (165 registers) beat two of them with
 // deeper buffers (467 us against 491) and one of 256 x 256 (518).  Measured at 8192 rows, 49152
-// ids, 576 columns, bf16: logits 467 us (993 TFLOP/s), d 525, both gradients 1057 (878
-// TFLOP/s); the library's single products of these shapes take 539, 604 and 750.
+// ids, 576 columns, bf16: logits 467 to 483 us (993 to 960 TFLOP/s), d 525 to 538, both
+// gradients 1057 to 1086 (878 to 854 TFLOP/s); the library's single products of these shapes
+// take 539, 604 and 750.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -311,10 +312,12 @@ __device__ __forceinline__ void lk_stage(const uint16_t* src, long stride, int p
 // 64 lanes of a wave, one candidate each: the end of the launch if its blocks go to the card's
 // places in turn, dE's first, and the shares' memory time.  Steps of the blocks that end last
 // count 0.73 us each (a block among others; with all places full a step's work adds 0.68 us
-// whatever the split), a share's float 1.7e-6 us, written and read; over 1 to 11 splits of the
-// three large cases the sum is within 8 % of what was measured, but for launches that leave
+// whatever the split), a share's float 1.7e-6 us, written and read; over 1 to 11 splits of
+// three large calls the sum is within 8 % of what was measured, but for launches that leave
 // most places empty.  (8192 rows, 16384 of the ids, 576 columns: 2 splits 362 us, 3 432, 4 376,
-// 5 433; a fixed number of blocks picked 4.)
+// 5 433; a fixed number of blocks picked 4.)  The 64 x 64 tiles take the same numbers, though
+// five of their blocks fit a CU and their steps are shorter: there they only keep any block from
+// being much longer than the others.
 __device__ int lk_choose(const LossArgs& a, int cnt, int lane) {
   const int nl = (cnt + a.bl - 1) / a.bl, nh = nl * a.nr, s = lane + 1;
   if (nh == 0) return 1;
@@ -593,7 +596,7 @@ __global__ void __launch_bounds__(WL * WR * 64, FINE ? 2 : 3) loss_logits_kernel
 }
 
 // dE's tiles (the first a.t2 blocks), then dh's: one launch, because neither fills the card
-// by itself (16384 ids and 576 columns: 384 tiles for 512 places) and dh's, split as finely
+// by itself (16384 ids and 576 columns: 384 tiles for 768 places) and dh's, split as finely
 // as one likes, fill the places that dE's leave.
 template <bool BF, int BL, int BR, int WL, int WR, int ST, bool FINE>
 __global__ void __launch_bounds__(WL * WR * 64, 3) loss_grad_kernel(LossArgs a) {
@@ -762,8 +765,14 @@ __global__ void __launch_bounds__(256) loss_dh_kernel(LossArgs a) {
 }
 
 // ---- plan ------------------------------------------------------------------------------
-// Big tiles (256 x 256, 8 waves) read 3 KB of LDS per 4 products; a few hundred rows leave
-// most of the card without one, so there 64 x 64 tiles of 4 waves run instead.
+// Big tiles, 128 x 256 for the logits and 128 x 192 for the gradients; a few hundred rows, or
+// few ids, leave most of the card without one (fewer than 256 squares of 256), so there 64 x 64
+// tiles run instead.  All have 4 waves.
+//
+// The gradients' tile is 192 of H's columns wide whatever H is.  At 576 and 960 columns that is
+// whole tiles (8192 rows of 49152 ids: 1080 and 1928 us, where 128 wide takes 1440 and 2275); at
+// 128, 256 and 384 a third, a third and nothing of the products is padding (775, 862 and 852 us
+// for 715, 735 and 818; 4773 rows of 8192 ids 122, 123 and 125 us for 104, 104 and 113).
 struct LossPlan {
   int Mp, Hp, small, fine, vtiles, piece, splits, want, most;
 };
