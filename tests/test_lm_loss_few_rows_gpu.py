@@ -41,3 +41,22 @@ def test_few_rows(N, V, H, kept, reduction, dtype):
         own = float((want.to(dtype).double() - want).norm())
         assert float((got.double() - want).norm()) <= 1.1 * own + 1e-6 * float(want.norm())
     assert not dh[~on].any()
+
+
+@pytest.mark.parametrize("N,V", [(61, 8192), (100, 70001)])
+def test_few_rows_each_gradient_alone_and_again(N, V):
+    """Only one input asks for a gradient, the backward runs twice: the same bits."""
+    from smsgate_amd.models import train_ops
+
+    g = torch.Generator(device=dev).manual_seed(N)
+    h = torch.randn(N, 256, generator=g, device=dev).bfloat16()
+    table = (torch.randn(V, 256, generator=g, device=dev) * 0.1).bfloat16()
+    labels = torch.randint(-1, V, (N,), generator=g, device=dev)
+    a, b = h.clone().requires_grad_(), table.clone().requires_grad_()
+    loss = train_ops.lm_loss(a, b, labels, ignore_index=-1)
+    want = torch.autograd.grad(loss, (a, b), retain_graph=True)
+    for x, y in zip(torch.autograd.grad(loss, (a, b)), want):
+        assert torch.equal(x, y)
+    a, b = h.clone().requires_grad_(), table.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(train_ops.lm_loss(a, table, labels, ignore_index=-1), a)[0], want[0])
+    assert torch.equal(torch.autograd.grad(train_ops.lm_loss(h, b, labels, ignore_index=-1), b)[0], want[1])
