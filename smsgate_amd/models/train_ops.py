@@ -52,6 +52,7 @@ from __future__ import annotations
 import contextlib
 import functools
 import math
+import operator
 import os
 from typing import Optional
 
@@ -323,8 +324,10 @@ def lm_loss(h: torch.Tensor, table: torch.Tensor, labels: torch.Tensor, *, reduc
             or ((N + 255) // 128) * ((V + 255) // 256) >= 1 << 24 or (N + V + 512) * (H + 63) >= 1 << 34:
         raise ValueError("lm_loss: 1 to 2^24 rows and ids, H a multiple of 8 up to 2^14, fewer than 2^24 tiles of "
                          "128 x 256, (rows + ids) * H under 2^34")
-    if not isinstance(ignore_index, int) or isinstance(ignore_index, bool):
-        raise TypeError("lm_loss: ignore_index must be a whole number")
+    try:
+        ignore_index = operator.index(ignore_index)
+    except TypeError:
+        raise TypeError("lm_loss: ignore_index must be a whole number") from None
     if not -(1 << 31) <= ignore_index < 1 << 31:
         raise ValueError("lm_loss: ignore_index must fit 32 bits")
     _on_gpu("lm_loss", h, table, labels)
